@@ -379,6 +379,48 @@ int32_t rlx_mla_append_attend(void *cache, int32_t layer, int32_t n_seqs, const 
                               const void *w_uk, const void *w_uv, float scale, int32_t mask_mode,
                               void *out, int32_t out_dtype);
 
+/* ---- trees of drafts: positions, attention, kept paths (no reference) ---- */
+/* Rotary positions: each of `heads` heads of `rows` rows rotated by the angles
+ * positions[row] * inv_freq[i], i < rotary_dim / 2, scaled by `scale`:
+ *   (x0, x1) -> scale (x0 cos a - x1 sin a, x0 sin a + x1 cos a)
+ * RLX_ROPE_PAIRS pairs dims (2i, 2i + 1), as rlx_gqa_project_append does;
+ * RLX_ROPE_HALVES dims (i, i + rotary_dim / 2).  Dims from rotary_dim (even, at
+ * most head_dim) on are copied.  positions (device int32 [rows], any value) and
+ * inv_freq (device f32) need no table, so a token may stand anywhere: a tree's
+ * node at context + depth.  Angles are reduced in 64 bits.  The gradient of the
+ * call is the call with negated positions.  x and out: device, head_dim
+ * consecutive elements a head, strides in elements (at least 0; out's rows and
+ * heads must not overlap); out may be x itself with its strides and type, and
+ * must not overlap it otherwise.  Runs on cache's stream (any handle). */
+#define RLX_ROPE_PAIRS 0
+#define RLX_ROPE_HALVES 1
+int32_t rlx_rope(void *cache, int64_t rows, int32_t heads, int32_t head_dim, int32_t rotary_dim,
+                 const void *x, int32_t x_dtype, int64_t x_row_stride, int64_t x_head_stride,
+                 const int32_t *positions, const float *inv_freq, float scale, int32_t pairing,
+                 void *out, int32_t out_dtype, int64_t out_row_stride, int64_t out_head_stride);
+/* Attention of a tree of drafted tokens.  The last n_nodes[i] (1 to 256) live
+ * tokens of sequence i are its tree's nodes in the order they were appended;
+ * parents (device int32, the sequences' entries one after the other) gives each
+ * node's parent as an index into its tree.  The last n_q[i] nodes (n_q NULL: all)
+ * are queries: a node attends every token before the tree, itself and its
+ * ancestors.  A parent outside [0, node) ends the chain (a root).  Values of
+ * nodes a query does not attend do not reach it, infinities and NaN included.
+ * q, out and the rest as for rlx_gqa_attend, but out must not overlap q.  f32
+ * queries, or f32 outputs, are computed to about 2^-17; bf16 both ways rounds
+ * the softmax weights to bf16. */
+int32_t rlx_gqa_attend_tree(void *cache, int32_t layer, int32_t n_seqs, const int32_t *seq_ids,
+                            const int32_t *n_nodes, const int32_t *n_q, int32_t num_heads,
+                            const void *q, int32_t q_dtype, int32_t qo_layout, float scale,
+                            const int32_t *parents, void *out, int32_t out_dtype);
+/* Keep an accepted path of each sequence's tree: of its last n_nodes[i] tokens
+ * (0 to 256) those at path[...] (host, n_keep[i] ascending indices a sequence,
+ * one sequence after the other) stay, moved together behind the tokens before
+ * the tree, and the rest is rolled back (layer -1: every layer).  Cache bytes,
+ * tables, free lists and append history are then those of an append of the kept
+ * tokens alone.  GQA caches.  Validated in full before any change. */
+int32_t rlx_keep_path(void *cache, int32_t layer, int32_t n_seqs, const int32_t *seq_ids,
+                      const int32_t *n_nodes, const int32_t *n_keep, const int32_t *path);
+
 /* ---- speculative rollback, eviction, compaction (no reference) -------- */
 /* Remove the last n_tokens[i] tokens of sequence seq_ids[i], in list order
  * (layer -1: every layer).  Pages left empty return to the free list, last
@@ -526,6 +568,33 @@ int32_t rlx_spec_accept_async(void *cache, const float *draft_logits, const floa
                               const int32_t *draft_tokens, const int32_t *n_draft, int32_t n_rows,
                               int32_t max_k, int32_t vocab, const float *uniforms,
                               const rlx_sampler_t *params, int32_t *n_accepted, int32_t *next_token);
+
+/* Acceptance of trees of drafts, for n_seqs sequences of n_nodes[i] (1 to 256,
+ * host) nodes.  Node 0 is the root, the last committed token; tokens and parents
+ * (device int32, the sequences one after the other) as for rlx_gqa_attend_tree,
+ * and row j of target_logits (device f32, target_stride elements apart) scores
+ * what follows node j.  The walk starts at the root; at a node with target
+ * distribution p (softmax at the sampler's temperature) its children are tried
+ * in order.  draft_logits (device f32 rows of the same nodes): the children were
+ * drawn from q = softmax(draft row) without replacement, and child c is accepted
+ * when uniforms[c] q(c) < p(c), else p becomes max(0, p - q) and q loses c, both
+ * rescaled.  draft_logits NULL: drafts chosen without a distribution; child c is
+ * accepted when uniforms[c] < p(c), else p loses c.  The walk goes on at an
+ * accepted child; where none is left the next token is drawn from p with
+ * uniforms[root].  Tokens so chosen are distributed as the target's own.
+ * A child whose token is outside [0, vocab), or that of an already rejected
+ * sibling, is passed over; a parent outside [0, node) makes a node unreachable.
+ * path (device int32 [n_seqs][path_stride], path_stride >= every n_nodes[i]):
+ * the accepted nodes from the root on, then -1; n_accepted and next_token device
+ * int32 [n_seqs].  Rows without probability mass (NaN) give some token of the
+ * vocabulary.  Sampler fields besides the temperature must be off
+ * (RLX_ERR_UNSUPPORTED).  Enqueued on the cache's stream without waiting. */
+int32_t rlx_tree_accept_async(void *cache, const float *target_logits, int64_t target_stride,
+                              const float *draft_logits, int64_t draft_stride, const int32_t *tokens,
+                              const int32_t *parents, int32_t n_seqs, const int32_t *n_nodes,
+                              int32_t vocab, const float *uniforms, const rlx_sampler_t *params,
+                              int32_t *path, int32_t path_stride, int32_t *n_accepted,
+                              int32_t *next_token);
 
 /* ---- state queries (synchronising) ------------------------------------ */
 /* Live token count; replaces TotalLen (kvcache.go:383-388). */

@@ -36,6 +36,8 @@ RLX_MASK_NONE = 2
 RLX_ROPE_OFFSET = 0
 RLX_ROPE_REF = 1
 RLX_ROPE_NONE = 2
+RLX_ROPE_PAIRS = 0
+RLX_ROPE_HALVES = 1
 RLX_TIME_ATTEND = 1
 RLX_TIME_PROJECT = 2
 RLX_TIME_SELECT = 4
@@ -98,6 +100,11 @@ SIGNATURES = {
                        _i32, _vp, _i32],
     "rlx_mla_append_attend": [_vp, _i32, _i32, _pi32, _pi32, _vp, _vp, _i32, _i32, _i32, _vp, _vp,
                               _i32, _vp, _vp, _f32, _i32, _vp, _i32],
+    "rlx_rope": [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _i64, _i64, _vp, _vp, _f32, _i32, _vp, _i32,
+                 _i64, _i64],
+    "rlx_gqa_attend_tree": [_vp, _i32, _i32, _pi32, _pi32, _pi32, _i32, _vp, _i32, _i32, _f32, _vp,
+                            _vp, _i32],
+    "rlx_keep_path": [_vp, _i32, _i32, _pi32, _pi32, _pi32, _pi32],
     "rlx_rollback": [_vp, _i32, _i32, _pi32, _pi32],
     "rlx_evict": [_vp, _i32, _i32, _pi32, _pi32],
     "rlx_compact": [_vp, _i32],
@@ -115,6 +122,8 @@ SIGNATURES = {
     "rlx_spec_accept_async": [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _psp, _vp, _vp],
     "rlx_spec_accept": [_vp, _vp, _vp, _pi32, _pi32, _i32, _i32, _i32, ctypes.POINTER(_f32), _psp,
                         _pi32, _pi32],
+    "rlx_tree_accept_async": [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _pi32, _i32, _vp, _psp, _vp,
+                              _i32, _vp, _vp],
     "rlx_seq_len": [_vp, _i32, _i32, _pi32],
     "rlx_seq_state": [_vp, _i32, _i32, _pi32],
     "rlx_page_table": [_vp, _i32, _i32, _pi32],

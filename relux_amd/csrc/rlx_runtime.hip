@@ -23,6 +23,7 @@
 #include <unistd.h>
 
 #include <map>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -30,6 +31,8 @@
 #include "rlx_common.h"
 #include "rlx_prefill_plan.h"
 #include "rlx_scratch.h"
+#include "rlx_tree.h"
+#include "rlx_tree_plan.h"
 
 using namespace rlx;
 
@@ -65,6 +68,16 @@ int32_t fail(int32_t code, const char *fmt, ...) {
         if (e_ != hipSuccess)                                                               \
             return fail(RLX_ERR_HIP, "%s failed: %s", #expr, hipGetErrorString(e_));        \
     } while (0)
+
+// A C entry whose host memory may run out: an error code instead of an exception.
+template <class F>
+int32_t guarded(F f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        return fail(RLX_ERR_HIP, "out of host memory");
+    }
+}
 
 enum Kind { kGQA = 0, kMLA = 1 };
 
@@ -2537,6 +2550,43 @@ static int32_t layer_range(Cache *c, int layer, int *lo, int *hi) {
     return RLX_OK;
 }
 
+// Drop the last n tokens of a sequence: emptied pages go back last first.
+static void drop_tail(Cache *c, int layer, int seq, int n_tokens) {
+    LayerState &ls = c->L[layer];
+    SeqState &s = ls.seqs[seq];
+    s.len -= n_tokens;
+    for (int n = n_tokens; n > 0;) {  // drop whole appends from the end
+        if (s.chunks.empty() || s.chunks.back() > n) {
+            s.chunks_ok = false;
+            break;
+        }
+        n -= s.chunks.back();
+        s.chunks.pop_back();
+    }
+    const int keep = (s.len + c->P - 1) / c->P;
+    for (int k = s.pages - 1; k >= keep; k--) {
+        ls.free_stack.push_back(c->entry(layer, seq, s.first + k));
+        c->set_entry(layer, seq, s.first + k, -1);
+    }
+    s.pages = keep;
+}
+
+// The append history after a tree of n tokens shrank to m kept ones: that of an
+// append of m tokens, where the tree was whole appends.
+static void keep_chunks(SeqState &s, int n, int m) {
+    if (n == m) return;
+    int sum = 0;
+    size_t k = s.chunks.size();
+    while (k > 0 && sum < n) sum += s.chunks[--k];
+    if (sum != n) {
+        s.chunks_ok = false;
+        return;
+    }
+    s.chunks.resize(k);
+    if (m > 0) s.chunks.push_back(m);
+    s.chunks.push_back(n - m);  // (drop_tail takes these off)
+}
+
 int32_t rlx_rollback(void *h, int32_t layer, int32_t n_seqs, const int32_t *seq_ids,
                      const int32_t *n_tokens) {
     if (!h) return fail(RLX_ERR_INVALID, "null cache");
@@ -2554,26 +2604,7 @@ int32_t rlx_rollback(void *h, int32_t layer, int32_t n_seqs, const int32_t *seq_
                             n_tokens[i], seq_ids[i], l, c->L[l].seqs[seq_ids[i]].len);
     }
     for (int i = 0; i < n_seqs; i++) {
-        const int seq = seq_ids[i];
-        for (int l = lo; l < hi; l++) {
-            LayerState &ls = c->L[l];
-            SeqState &s = ls.seqs[seq];
-            s.len -= n_tokens[i];
-            for (int n = n_tokens[i]; n > 0;) {  // drop whole appends from the end
-                if (s.chunks.empty() || s.chunks.back() > n) {
-                    s.chunks_ok = false;
-                    break;
-                }
-                n -= s.chunks.back();
-                s.chunks.pop_back();
-            }
-            const int keep = (s.len + c->P - 1) / c->P;
-            for (int k = s.pages - 1; k >= keep; k--) {
-                ls.free_stack.push_back(c->entry(l, seq, s.first + k));
-                c->set_entry(l, seq, s.first + k, -1);
-            }
-            s.pages = keep;
-        }
+        for (int l = lo; l < hi; l++) drop_tail(c, l, seq_ids[i], n_tokens[i]);
     }
     return RLX_OK;
 }
@@ -3171,6 +3202,310 @@ int32_t rlx_spec_accept(void *h, const float *draft_logits, const float *target_
     HIP_TRY(hipMemcpyAsync(next_token, a.next, (size_t)n_rows * 4, hipMemcpyDeviceToHost, c->stream));
     HIP_TRY(hipStreamSynchronize(c->stream));
     return RLX_OK;
+}
+
+// ---- trees of drafts ---------------------------------------------------------
+
+static bool is_dtype(int32_t t) { return t == RLX_F32 || t == RLX_BF16; }
+
+int32_t rlx_rope(void *h, int64_t rows, int32_t heads, int32_t head_dim, int32_t rotary_dim, const void *x,
+                 int32_t x_dtype, int64_t x_row_stride, int64_t x_head_stride, const int32_t *positions,
+                 const float *inv_freq, float scale, int32_t pairing, void *out, int32_t out_dtype,
+                 int64_t out_row_stride, int64_t out_head_stride) {
+    if (!h) return fail(RLX_ERR_INVALID, "null cache");
+    Cache *c = as_cache(h);
+    if (rows < 0 || heads < 0 || head_dim <= 0 || rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2)
+        return fail(RLX_ERR_INVALID, "rlx_rope: rows=%lld heads=%d head_dim=%d rotary_dim=%d", (long long)rows, heads,
+                    head_dim, rotary_dim);
+    if (!is_dtype(x_dtype) || !is_dtype(out_dtype)) return fail(RLX_ERR_INVALID, "rlx_rope: dtype");
+    if (pairing != RLX_ROPE_PAIRS && pairing != RLX_ROPE_HALVES) return fail(RLX_ERR_INVALID, "rlx_rope: pairing");
+    if (rows == 0 || heads == 0) return RLX_OK;
+    if (!x || !out || (rotary_dim > 0 && (!positions || !inv_freq)))
+        return fail(RLX_ERR_INVALID, "rlx_rope: null pointer");
+    // Rows and heads must not overlap in the output: heads within a row, or rows within a head.
+    const auto apart = [&](int64_t rs, int64_t hs) {
+        if (rs < 0 || hs < 0) return false;
+        const bool h_in = heads == 1 || hs >= head_dim, r_in = rows == 1 || rs >= head_dim;
+        return h_in && r_in && (rows == 1 || heads == 1 || rs >= (heads - 1) * hs + head_dim ||
+                                hs >= (rows - 1) * rs + head_dim);
+    };
+    if (!apart(out_row_stride, out_head_stride) || x_row_stride < 0 || x_head_stride < 0)
+        return fail(RLX_ERR_INVALID, "rlx_rope: strides of x (%lld, %lld), out (%lld, %lld)", (long long)x_row_stride,
+                    (long long)x_head_stride, (long long)out_row_stride, (long long)out_head_stride);
+    const bool same = x == out && x_dtype == out_dtype && x_row_stride == out_row_stride &&
+                      x_head_stride == out_head_stride;
+    const auto span = [&](int64_t rs, int64_t hs, int32_t t) {
+        return (size_t)((rows - 1) * rs + (heads - 1) * hs + head_dim) * (t == RLX_BF16 ? 2 : 4);
+    };
+    const char *xb = (const char *)x, *ob = (const char *)out;
+    if (!same && xb < ob + span(out_row_stride, out_head_stride, out_dtype) &&
+        ob < xb + span(x_row_stride, x_head_stride, x_dtype))
+        return fail(RLX_ERR_INVALID, "rlx_rope: x and out overlap and are not the same rows");
+    RopeArgs a{};
+    a.x = x;
+    a.out = out;
+    a.x_row = x_row_stride;
+    a.x_head = x_head_stride;
+    a.out_row = out_row_stride;
+    a.out_head = out_head_stride;
+    a.pos = positions;
+    a.inv_freq = inv_freq;
+    a.scale = scale;
+    a.rows = rows;
+    a.heads = heads;
+    a.D = head_dim;
+    a.rd = rotary_dim;
+    a.x_bf16 = x_dtype == RLX_BF16;
+    a.out_bf16 = out_dtype == RLX_BF16;
+    a.halves = pairing == RLX_ROPE_HALVES;
+    HIP_TRY(launch_rope(c->stream, a, c->cus));
+    return RLX_OK;
+}
+
+static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const int32_t *seq_ids,
+                                const int32_t *n_nodes, const int32_t *n_q, int32_t num_heads, const void *q,
+                                int32_t q_dtype, int32_t qo_layout, float scale, const int32_t *parents, void *out,
+                                int32_t out_dtype) {
+    const int G = num_heads / c->kvh;
+    const bool fine = q_dtype == RLX_F32 || out_dtype == RLX_F32;
+    int max_qr = 0;
+    for (int i = 0; i < n_seqs; i++) max_qr = std::max(max_qr, G * (n_q ? n_q[i] : n_nodes[i]));
+    const int qt = tree_tile_rows(c->hd, max_qr, fine);
+    std::vector<TreeRow> rows(n_seqs);
+    std::vector<TreeLoad> load(n_seqs);
+    int qrow = 0, node0 = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        const SeqState &s = c->L[layer].seqs[seq_ids[i]];
+        const int nq = n_q ? n_q[i] : n_nodes[i];
+        TreeRow &r = rows[i];
+        r.tab = (int32_t)(c->row_base(layer, seq_ids[i]) + s.first);
+        r.len = s.len;
+        r.nodes = n_nodes[i] | nq << 16;
+        r.qrow = qrow;
+        r.node0 = node0;
+        load[i] = TreeLoad{s.len, (nq * G + qt - 1) / qt, nq * G};
+        qrow += nq;
+        node0 += n_nodes[i];
+    }
+    const std::vector<int> cuts = tree_cuts(load, c->kvh, c->cus, qt, c->hd, fine);
+    int64_t wgs = 0, parts = 0;
+    bool merge = false;
+    for (int i = 0; i < n_seqs; i++) {
+        const int64_t n = (int64_t)load[i].tiles * c->kvh * cuts[i];
+        rows[i].nsplit = cuts[i];
+        rows[i].wg0 = (int32_t)wgs;
+        rows[i].part = (int32_t)parts;
+        wgs += n;
+        if (cuts[i] > 1) {
+            parts += n;
+            merge = true;
+        }
+    }
+    if (wgs > 0x7FFFFFFF) return fail(RLX_ERR_UNSUPPORTED, "rlx_gqa_attend_tree: %lld work-groups", (long long)wgs);
+    int32_t rc;
+    if ((rc = flush_patches(c))) return rc;
+    const size_t po = (size_t)parts * qt * c->hd * sizeof(float), pm = (size_t)parts * qt * 2 * sizeof(float);
+    if ((rc = ensure_ws(c, po + pm))) return rc;
+    PlanArg plan;
+    TreeArgs a{};
+    if (rows.size() * sizeof(TreeRow) <= sizeof plan) {
+        memcpy(plan.b, rows.data(), rows.size() * sizeof(TreeRow));
+    } else {
+        std::vector<int32_t> work((size_t)wgs);
+        for (int i = 0, w = 0; i < n_seqs; i++)
+            for (int k = load[i].tiles * c->kvh * cuts[i]; k > 0; k--) work[w++] = i;
+        Blob b;
+        const size_t o_r = b.add(rows), o_w = b.add(work);
+        void *dev;
+        if ((rc = stage(c, b.bytes.data(), b.bytes.size(), &dev))) return rc;
+        a.rows = (const TreeRow *)((char *)dev + o_r);
+        a.work = (const int32_t *)((char *)dev + o_w);
+    }
+    a.kpool = c->L[layer].pool0;
+    a.vpool = c->L[layer].pool1;
+    a.table = c->d_table;
+    a.parents = parents;
+    a.q = q;
+    a.out = out;
+    a.part_o = (float *)c->ws.ptr;
+    a.part_ml = (float *)((char *)c->ws.ptr + po);
+    a.n_rows = n_seqs;
+    a.H = num_heads;
+    a.KVH = c->kvh;
+    a.DQ = c->hdi;
+    a.P = c->P;
+    a.pshift = (c->P & (c->P - 1)) == 0 ? __builtin_ctz((unsigned)c->P) : -1;
+    a.q_bf16 = q_dtype == RLX_BF16;
+    a.out_bf16 = out_dtype == RLX_BF16;
+    a.layout = qo_layout;
+    if (!(scale > 0.f)) scale = (float)(1.0 / std::sqrt((double)c->hdu));
+    a.qscale = scale * 1.4426950408889634f;
+    hipEvent_t e0, e1;
+    if ((rc = timing_events(c, &e0, &e1))) return rc;
+    HIP_TRY(launch_tree_attend(c->stream, plan, a, c->hd, qt, fine, (int)wgs, merge, max_qr, e0, e1));
+    return RLX_OK;
+}
+
+int32_t rlx_gqa_attend_tree(void *h, int32_t layer, int32_t n_seqs, const int32_t *seq_ids, const int32_t *n_nodes,
+                            const int32_t *n_q, int32_t num_heads, const void *q, int32_t q_dtype, int32_t qo_layout,
+                            float scale, const int32_t *parents, void *out, int32_t out_dtype) {
+    if (!h) return fail(RLX_ERR_INVALID, "null cache");
+    return guarded([&]() -> int32_t {
+        Cache *c = as_cache(h);
+        int32_t rc = check_gqa_attend(c, layer, n_seqs, seq_ids, num_heads, q_dtype, qo_layout, RLX_MASK_CAUSAL,
+                                      out_dtype);
+        if (rc) return rc;
+        if (n_seqs == 0) return RLX_OK;
+        if (!q || !out || !parents || !n_nodes) return fail(RLX_ERR_INVALID, "null q/out/parents/n_nodes");
+        int64_t rows = 0, nodes = 0;
+        for (int i = 0; i < n_seqs; i++) {
+            const int len = c->L[layer].seqs[seq_ids[i]].len, nq = n_q ? n_q[i] : n_nodes[i];
+            if (n_nodes[i] < 1 || n_nodes[i] > kTreeMaxNodes)
+                return fail(RLX_ERR_UNSUPPORTED, "n_nodes=%d must be in [1, %d]", n_nodes[i], kTreeMaxNodes);
+            if (n_nodes[i] > len)
+                return fail(RLX_ERR_STATE, "a tree of %d nodes on sequence %d holding %d tokens", n_nodes[i],
+                            seq_ids[i], len);
+            if (nq < 1 || nq > n_nodes[i])
+                return fail(RLX_ERR_INVALID, "n_q=%d must be in [1, n_nodes=%d]", nq, n_nodes[i]);
+            rows += nq;
+            nodes += n_nodes[i];
+        }
+        if (rows * num_heads > 0x7FFFFFFF || nodes > 0x7FFFFFFF)
+            return fail(RLX_ERR_UNSUPPORTED, "%lld query rows of %d heads", (long long)rows, num_heads);
+        if (qo_overlap((size_t)rows, q, q_dtype, out, out_dtype, num_heads * c->hdu))
+            return fail(RLX_ERR_INVALID, "rlx_gqa_attend_tree: q and out overlap");
+        return gqa_call_padded(c, rows * num_heads, q, q_dtype, out, out_dtype, [&](const void *qk, void *ok) {
+            return attend_tree_impl(c, layer, n_seqs, seq_ids, n_nodes, n_q, num_heads, qk, q_dtype, qo_layout, scale,
+                                    parents, ok, out_dtype);
+        });
+    });
+}
+
+int32_t rlx_keep_path(void *h, int32_t layer, int32_t n_seqs, const int32_t *seq_ids, const int32_t *n_nodes,
+                      const int32_t *n_keep, const int32_t *path) {
+    if (!h) return fail(RLX_ERR_INVALID, "null cache");
+    return guarded([&]() -> int32_t {
+        Cache *c = as_cache(h);
+        if (c->kind != kGQA) return fail(RLX_ERR_INVALID, "rlx_keep_path on an MLA cache");
+        int lo, hi;
+        int32_t rc = layer_range(c, layer, &lo, &hi);
+        if (rc) return rc;
+        if ((rc = check_seqs(c, n_seqs, seq_ids))) return rc;
+        if (n_seqs > 0 && (!n_nodes || !n_keep)) return fail(RLX_ERR_INVALID, "null node counts");
+        std::vector<KeepRow> rows;
+        std::vector<int32_t> moves;
+        for (int i = 0, at = 0; i < n_seqs; at += n_keep[i], i++) {
+            const int n = n_nodes[i], m = n_keep[i];
+            if (n < 0 || n > kTreeMaxNodes)
+                return fail(RLX_ERR_UNSUPPORTED, "n_nodes=%d must be in [0, %d]", n, kTreeMaxNodes);
+            if (m < 0 || m > n) return fail(RLX_ERR_INVALID, "n_keep=%d must be in [0, n_nodes=%d]", m, n);
+            if (m > 0 && !path) return fail(RLX_ERR_INVALID, "null path");
+            for (int j = 0; j < m; j++)
+                if (path[at + j] < 0 || path[at + j] >= n || (j && path[at + j] <= path[at + j - 1]))
+                    return fail(RLX_ERR_INVALID, "path of sequence %d: node %d at place %d (ascending, below %d)",
+                                seq_ids[i], path[at + j], j, n);
+            for (int l = lo; l < hi; l++)
+                if (n > c->L[l].seqs[seq_ids[i]].len)
+                    return fail(RLX_ERR_STATE, "a tree of %d nodes on seq %d, layer %d holding %d", n, seq_ids[i], l,
+                                c->L[l].seqs[seq_ids[i]].len);
+            int p0 = 0;  // the beginning that stays where it is
+            while (p0 < m && path[at + p0] == p0) p0++;
+            if (p0 == m) continue;
+            for (int l = lo; l < hi; l++) {
+                const SeqState &s = c->L[l].seqs[seq_ids[i]];
+                rows.push_back(KeepRow{c->L[l].pool0, c->L[l].pool1, (int32_t)(c->row_base(l, seq_ids[i]) + s.first),
+                                       s.len - n + p0, m - p0, (int32_t)moves.size()});
+            }
+            for (int j = p0; j < m; j++) moves.push_back(path[at + j] - p0);
+        }
+        if (!rows.empty()) {
+            if ((rc = flush_patches(c))) return rc;
+            Blob b;
+            const size_t o_r = b.add(rows), o_p = b.add(moves);
+            PlanArg plan;
+            if (b.bytes.size() <= sizeof plan) {
+                memcpy(plan.b, b.bytes.data(), b.bytes.size());
+                HIP_TRY(launch_tree_keep(c->stream, &plan, nullptr, nullptr, (int)o_p, (int)rows.size(), c->d_table,
+                                         c->kvh, c->hd, c->P));
+            } else {
+                void *dev;
+                if ((rc = stage(c, b.bytes.data(), b.bytes.size(), &dev))) return rc;
+                HIP_TRY(launch_tree_keep(c->stream, nullptr, (const KeepRow *)((char *)dev + o_r),
+                                         (const int32_t *)((char *)dev + o_p), 0, (int)rows.size(), c->d_table, c->kvh,
+                                         c->hd, c->P));
+            }
+        }
+        // The state of an append of the kept tokens alone.
+        for (int i = 0; i < n_seqs; i++)
+            for (int l = lo; l < hi; l++) {
+                SeqState &s = c->L[l].seqs[seq_ids[i]];
+                const int m = n_keep[i];
+                keep_chunks(s, n_nodes[i], m);
+                drop_tail(c, l, seq_ids[i], n_nodes[i] - m);
+            }
+        return RLX_OK;
+    });
+}
+
+int32_t rlx_tree_accept_async(void *h, const float *target_logits, int64_t target_stride, const float *draft_logits,
+                              int64_t draft_stride, const int32_t *tokens, const int32_t *parents, int32_t n_seqs,
+                              const int32_t *n_nodes, int32_t vocab, const float *uniforms, const rlx_sampler_t *p,
+                              int32_t *path, int32_t path_stride, int32_t *n_accepted, int32_t *next_token) {
+    if (!h) return fail(RLX_ERR_INVALID, "null cache");
+    return guarded([&]() -> int32_t {
+        Cache *c = as_cache(h);
+        if (n_seqs < 0 || vocab <= 0 || !p || target_stride < vocab || (draft_logits && draft_stride < vocab))
+            return fail(RLX_ERR_INVALID, "rlx_tree_accept_async: n_seqs=%d vocab=%d strides %lld, %lld", n_seqs, vocab,
+                        (long long)target_stride, (long long)draft_stride);
+        if (vocab > 1 << 30) return fail(RLX_ERR_UNSUPPORTED, "rlx_tree_accept_async: vocab %d", vocab);
+        if ((p->top_k > 0 && p->top_k < vocab) || (p->top_p > 0.f && p->top_p < 1.f) || p->min_p > 0.f ||
+            (p->repeat_penalty != 0.f && p->repeat_penalty != 1.f) || p->frequency_penalty != 0.f ||
+            p->presence_penalty != 0.f)
+            return fail(RLX_ERR_UNSUPPORTED, "rlx_tree_accept_async: sampler fields besides the temperature are set");
+        if (n_seqs == 0) return RLX_OK;
+        if (!target_logits || !tokens || !parents || !n_nodes || !uniforms || !path || !n_accepted || !next_token)
+            return fail(RLX_ERR_INVALID, "rlx_tree_accept_async: null pointer");
+        std::vector<int2> trees(n_seqs);
+        int64_t at = 0;
+        for (int i = 0; i < n_seqs; i++) {
+            if (n_nodes[i] < 1 || n_nodes[i] > kTreeMaxNodes)
+                return fail(RLX_ERR_UNSUPPORTED, "n_nodes=%d must be in [1, %d]", n_nodes[i], kTreeMaxNodes);
+            if (n_nodes[i] > path_stride)
+                return fail(RLX_ERR_INVALID, "path rows of %d entries for a tree of %d nodes", path_stride, n_nodes[i]);
+            trees[i] = int2{(int)at, n_nodes[i]};
+            at += n_nodes[i];
+        }
+        if (at > 0x7FFFFFFF) return fail(RLX_ERR_UNSUPPORTED, "rlx_tree_accept_async: %lld nodes", (long long)at);
+        TreeAcceptArgs a{};
+        PlanArg plan;
+        const bool args = trees.size() * sizeof(int2) <= sizeof plan;
+        if (args) {
+            memcpy(plan.b, trees.data(), trees.size() * sizeof(int2));
+        } else {
+            void *dev;
+            const int32_t rc = stage(c, trees.data(), trees.size() * sizeof(int2), &dev);
+            if (rc) return rc;
+            a.trees = (const int2 *)dev;
+        }
+        a.t_logits = target_logits;
+        a.d_logits = draft_logits;
+        a.t_stride = target_stride;
+        a.d_stride = draft_stride;
+        a.tok = tokens;
+        a.parents = parents;
+        a.u = uniforms;
+        a.V = vocab;
+        a.temperature = p->temperature > 0.f ? p->temperature : 1e-5f;
+        a.path = path;
+        a.n_acc = n_accepted;
+        a.next = next_token;
+        a.path_stride = path_stride;
+        hipEvent_t e0, e1;
+        int32_t rc;
+        if ((rc = timing_events(c, &e0, &e1, RLX_TIME_SELECT))) return rc;
+        HIP_TRY(launch_tree_accept(c->stream, args ? &plan : nullptr, a, n_seqs, e0, e1));
+        return RLX_OK;
+    });
 }
 
 int32_t rlx_pool_ptr(void *h, int32_t layer, void **k_pool, void **v_pool) {

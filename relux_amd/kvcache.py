@@ -17,8 +17,10 @@ import torch
 from . import _lib
 from ._lib import check, i32_array
 
+MAX_TREE_NODES = 256  # nodes of one sequence's tree of drafts
 _MASKS = {"causal": _lib.RLX_MASK_CAUSAL, "ref": _lib.RLX_MASK_REF, "none": _lib.RLX_MASK_NONE}
 _LAYOUTS = {"HSD": _lib.RLX_LAYOUT_HSD, "SHD": _lib.RLX_LAYOUT_SHD}
+_PAIRING = {"pairs": _lib.RLX_ROPE_PAIRS, "halves": _lib.RLX_ROPE_HALVES}
 _ROPE = {"offset": _lib.RLX_ROPE_OFFSET, "ref": _lib.RLX_ROPE_REF, "none": _lib.RLX_ROPE_NONE}
 
 
@@ -43,6 +45,14 @@ def _dev(t, what):
         raise TypeError(f"{what} must be a GPU torch tensor")
     if not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def _ints(t, n, what, device):
+    """A contiguous int32 tensor of n entries on `device`."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.numel() != n \
+            or not t.is_contiguous():
+        raise TypeError(f"{what} must be a contiguous int32 tensor of {n} entries on {device}")
     return ctypes.c_void_p(t.data_ptr())
 
 
@@ -213,6 +223,38 @@ class _PagedCache:
                                         _dev(out, "out"), _dtype_code(out)))
         return out
 
+    def Rotate(self, x, positions, inv_freq, layout="pairs", scale=1.0, out=None):
+        """Rotary positions on this cache's stream (rlx_rope): x [rows][heads]
+        [head_dim] (f32 or bf16, unit stride along head_dim, any others) with row
+        r turned by positions[r] * inv_freq -- positions int32 [rows] of any
+        value, inv_freq f32 [rotary_dim / 2] as rope_frequencies gives them, so
+        rotary_dim is their number twice and further dims are copied.  layout
+        "pairs": dims (2i, 2i + 1); "halves": dims (i, i + rotary_dim / 2).  out:
+        a tensor of x's shape, x itself to rotate in place; None: a new one.
+        The gradient is Rotate of the output's gradient by -positions."""
+        if layout not in _PAIRING:
+            raise ValueError(f"layout must be one of {sorted(_PAIRING)}")
+        if not isinstance(x, torch.Tensor) or x.dim() != 3:
+            raise ValueError("x must be a [rows][heads][head_dim] tensor")
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        for t, what in ((x, "x"), (out, "out")):
+            if not isinstance(t, torch.Tensor) or t.device != self.device:
+                raise TypeError(f"{what} must be a tensor on {self.device}")
+            if t.shape != x.shape or (t.shape[2] > 1 and t.stride(2) != 1):
+                raise ValueError(f"{what} must be [rows][heads][head_dim] with unit stride along head_dim")
+        rows, heads, head_dim = x.shape
+        if not isinstance(inv_freq, torch.Tensor) or inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 \
+                or inv_freq.device != self.device or not inv_freq.is_contiguous():
+            raise TypeError("inv_freq must be a contiguous float32 vector on the cache's device")
+        if 2 * inv_freq.numel() > head_dim:
+            raise ValueError(f"{inv_freq.numel()} frequencies for {head_dim} dims")
+        check(self._lib.rlx_rope(self._h, rows, heads, head_dim, 2 * inv_freq.numel(), x.data_ptr(), _dtype_code(x),
+                                 x.stride(0), x.stride(1), _ints(positions, rows, "positions", self.device),
+                                 inv_freq.data_ptr(), float(scale), _PAIRING[layout], out.data_ptr(),
+                                 _dtype_code(out), out.stride(0), out.stride(1)))
+        return out
+
     def _lens(self, layer_idx, seq_ids):
         return [self.TotalLen(layer_idx, s) for s in seq_ids]
 
@@ -377,6 +419,56 @@ class KVCache(_PagedCache):
         return out
 
 
+    def AttendTree(self, layer_idx, q, num_heads, parents, seq_ids=(0,), n_nodes=None, n_q=None, layout="SHD",
+                   scale=None, out=None, out_dtype=torch.float32):
+        """Attention of trees of drafted tokens (rlx_gqa_attend_tree).  The last
+        n_nodes[i] live tokens of sequence i are its tree's nodes in the order
+        they were appended, parents (device int32, one entry a node, the
+        sequences one after the other) the index of each node's parent in its
+        tree (-1: none).  The last n_q[i] nodes (default: all) are queries; each
+        attends the tokens before the tree, itself and its ancestors.  q: rows x
+        num_heads x head_dim in `layout`; out must not share q's memory."""
+        seq_ids = list(seq_ids)
+        if n_nodes is None:
+            if len(seq_ids) != 1 or not isinstance(parents, torch.Tensor):
+                raise ValueError("n_nodes is required for several sequences")
+            n_nodes = [parents.numel()]
+        n_nodes = list(n_nodes)
+        n_q = n_nodes if n_q is None else list(n_q)
+        if len(n_nodes) != len(seq_ids) or len(n_q) != len(seq_ids):
+            raise ValueError("n_nodes and n_q need one entry per sequence")
+        for n, m in zip(n_nodes, n_q):
+            if not 1 <= m <= n <= MAX_TREE_NODES:
+                raise ValueError(f"{m} queries of {n} nodes: 1 <= n_q <= n_nodes <= {MAX_TREE_NODES}")
+        if q.numel() != sum(n_q) * num_heads * self.head_dim:
+            raise ValueError("q size does not match sum(n_q) x num_heads x head_dim")
+        if out is None:
+            out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+        if out.numel() != q.numel():
+            raise ValueError("out must have q's size")
+        for t, what in ((q, "q"), (out, "out")):
+            if t.device != self.device:
+                raise TypeError(f"{what} must be a tensor on {self.device}")
+        check(self._lib.rlx_gqa_attend_tree(
+            self._h, layer_idx, len(seq_ids), i32_array(seq_ids), i32_array(n_nodes), i32_array(n_q), num_heads,
+            _dev(q, "q"), _dtype_code(q), _LAYOUTS[layout], float(scale or 0.0),
+            _ints(parents, sum(n_nodes), "parents", self.device), _dev(out, "out"), _dtype_code(out)))
+        return out
+
+    def KeepPath(self, seq, n_nodes, path, layer=-1):
+        """Of the last n_nodes tokens of `seq`, a tree's nodes, keep those of
+        `path` (ascending node indices, the root first) and roll the others back
+        (rlx_keep_path): the cache is then as if the kept tokens alone had been
+        appended.  With lists, of every listed sequence in one call."""
+        if isinstance(seq, (list, tuple)):
+            seqs, ns, paths = list(seq), list(n_nodes), [list(p) for p in path]
+        else:
+            seqs, ns, paths = [seq], [n_nodes], [list(path)]
+        if len(ns) != len(seqs) or len(paths) != len(seqs):
+            raise ValueError("n_nodes and path need one entry per sequence")
+        check(self._lib.rlx_keep_path(self._h, layer, len(seqs), i32_array(seqs), i32_array(ns),
+                                      i32_array([len(p) for p in paths]), i32_array(sum(paths, []))))
+
     def ProjectAppend(self, layer_idx, x, w_packed, num_heads, rope=None, seq_ids=(0,), n_tok=None,
                       rope_mode="offset", q_dtype=torch.float32):
         """Fused pre-attention step (mha.go:250-289): q/k/v projection of the
@@ -455,6 +547,45 @@ def rope_tables(head_dim, base, max_seq, device):
     cos_t = np.cos(angle.astype(np.float64)).astype(np.float32)
     sin_t = np.sin(angle.astype(np.float64)).astype(np.float32)
     return (torch.from_numpy(cos_t).to(device), torch.from_numpy(sin_t).to(device))
+
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling=None, device="cpu"):
+    """inv_freq (f32 [rotary_dim / 2] on `device`) and the scale for Rotate:
+    base^(-2i / rotary_dim), stretched to longer contexts by `scaling`:
+
+      {"type": "linear", "factor": s}    every frequency / s
+      {"type": "ntk", "factor": s}       base * s^(rotary_dim / (rotary_dim - 2)):
+                                         the slowest / s, the fastest as it was
+      {"type": "yarn", "factor": s, "original": n, "fast": 32, "slow": 1}
+                                         dims that turn more than `fast` times in
+                                         the n original positions stay, fewer than
+                                         `slow` times are divided by s, a ramp in
+                                         between; scale 0.1 ln(s) + 1
+    """
+    import numpy as np
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim={rotary_dim} must be even and positive")
+    kind = scaling["type"] if scaling else None
+    factor = float(scaling["factor"]) if scaling else 1.0
+    if kind not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"scaling type {kind!r}")
+    if not factor >= 1.0 or not base > 1.0:
+        raise ValueError(f"factor={factor} must be at least 1, base={base} above 1")
+    if kind == "ntk":
+        base = base * factor ** (rotary_dim / max(rotary_dim - 2, 1))
+    i = np.arange(rotary_dim // 2, dtype=np.float64)
+    inv, scale = base ** (-2.0 * i / rotary_dim), 1.0
+    if kind == "linear":
+        inv = inv / factor
+    elif kind == "yarn":
+        def dim(turns):  # the dim whose pair turns that often in the original positions
+            return rotary_dim * math.log(scaling["original"] / (turns * 2 * math.pi)) / (2 * math.log(base))
+        lo = max(math.floor(dim(scaling.get("fast", 32))), 0)
+        hi = min(math.ceil(dim(scaling.get("slow", 1))), rotary_dim - 1)
+        ramp = np.clip((i - lo) / max(hi - lo, 1e-3), 0.0, 1.0)
+        inv = inv / factor * ramp + inv * (1.0 - ramp)
+        scale = 0.1 * math.log(factor) + 1.0
+    return torch.from_numpy(inv.astype(np.float32)).to(device), scale
 
 
 class MLACache(_PagedCache):

@@ -16,6 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import SamplerParams, check
+from .kvcache import MAX_TREE_NODES
 
 
 class Draws:
@@ -183,6 +184,66 @@ def spec_accept_async(cache, draft_logits, target_logits, draft_tokens, n_draft,
                                             n_acc.data_ptr(), next_tok.data_ptr()))
     return n_acc, next_tok
 
+
+def tree_accept_async(cache, target_logits, tokens, parents, n_nodes, uniforms, sampler, draft_logits=None,
+                      path=None, n_acc=None, next_tok=None):
+    """Acceptance of trees of drafts on device state (rlx_tree_accept_async).
+    n_nodes: nodes of each sequence's tree (host ints); tokens, parents int32 and
+    uniforms f32, one entry a node, the sequences one after the other; node 0 is
+    the root, the last committed token.  target_logits [nodes, V] f32: row j
+    scores what follows node j; draft_logits the rows of the same nodes that the
+    children were drawn from, in order and without replacement, or None for
+    drafts chosen without a distribution.  Returns (or fills) (path [B, max
+    n_nodes] -- the accepted nodes, root first, then -1 --, n_acc [B], next [B])
+    int32 device tensors; enqueued on the cache's stream without waiting.  Of
+    the sampler the temperature counts; its other fields must be off."""
+    n_nodes = [int(n) for n in n_nodes]
+    B, rows, wide = len(n_nodes), sum(n_nodes), max(n_nodes, default=0)
+    dev = cache.device
+    for n in n_nodes:
+        if not 1 <= n <= MAX_TREE_NODES:
+            raise ValueError(f"{n} nodes: trees have 1 to {MAX_TREE_NODES}")
+    for name, x in (("target_logits", target_logits), ("draft_logits", draft_logits)):
+        if x is None and name == "draft_logits":
+            continue
+        if not isinstance(x, torch.Tensor) or x.device != dev or x.dtype != torch.float32:
+            raise TypeError(f"{name} must be a float32 tensor on {dev}")
+        if x.dim() != 2 or x.shape[0] != rows or x.stride(1) != 1 or x.shape[1] != target_logits.shape[1]:
+            raise ValueError(f"{name} must be [{rows}][vocab] with unit stride along the vocabulary")
+    if path is None:
+        path = torch.empty(B, wide, dtype=torch.int32, device=dev)
+    if n_acc is None:
+        n_acc = torch.empty(B, dtype=torch.int32, device=dev)
+    if next_tok is None:
+        next_tok = torch.empty(B, dtype=torch.int32, device=dev)
+    if path.dim() != 2 or path.shape[0] != B or path.shape[1] < wide:
+        raise ValueError(f"path must be [{B}][{wide} or more]")
+    checks = (("tokens", tokens, torch.int32, rows), ("parents", parents, torch.int32, rows),
+              ("uniforms", uniforms, torch.float32, rows), ("n_acc", n_acc, torch.int32, B),
+              ("next_tok", next_tok, torch.int32, B), ("path", path, torch.int32, B * path.shape[1]))
+    for name, x, dt, n in checks:
+        if not isinstance(x, torch.Tensor) or x.device != dev or x.dtype != dt or x.numel() != n \
+                or not x.is_contiguous():
+            raise TypeError(f"{name} must be a contiguous {dt} tensor of {n} entries on {dev}")
+    p = sampler.params()
+    d = draft_logits
+    check(_lib.load().rlx_tree_accept_async(
+        cache._h, target_logits.data_ptr(), target_logits.stride(0), None if d is None else d.data_ptr(),
+        0 if d is None else d.stride(0), tokens.data_ptr(), parents.data_ptr(), B, _lib.i32_array(n_nodes),
+        target_logits.shape[1], uniforms.data_ptr(), ctypes.byref(p), path.data_ptr(), path.shape[1],
+        n_acc.data_ptr(), next_tok.data_ptr()))
+    return path, n_acc, next_tok
+
+
+def tree_accept(cache, target_logits, tokens, parents, n_nodes, uniforms, sampler, draft_logits=None):
+    """tree_accept_async, waited for: (accepted path of each sequence as a list
+    of nodes, the root first -- KeepPath's argument --, next tokens)."""
+    path, n_acc, nxt = tree_accept_async(cache, target_logits, tokens, parents, n_nodes, uniforms, sampler,
+                                         draft_logits)
+    cache.Sync()
+    return [p[:a + 1] for p, a in zip(path.tolist(), n_acc.tolist())], nxt.tolist()
+
+
 def spec_draws_used(n_acc, k):
     """Draws acceptPhase consumes: a test per draft up to the first
     rejection, then one for the resample or the final Sample."""
@@ -249,4 +310,93 @@ class SpeculativeDecoder:
             gen += toks[:n_acc] + [nxt]
             drafted += k
             accepted += n_acc
+        return gen[:max_new], (accepted / drafted if drafted else 0.0)
+
+
+class TreeSpeculativeDecoder:
+    """Speculative decoding with a tree of drafts: `branch` children a level
+    along each of the level's most likely nodes, one target call for the whole
+    tree, acceptance with the target's own distribution (tree_accept) and the
+    accepted path kept in both caches (KeepPath).
+
+    draft / target: model objects with
+      forward(ids) -> f32 device logits [len(ids), vocab], appending to the
+        model's own KVCache (`model.cache`);
+      forward_tree(ids, parents, depths, n_new) -> f32 device logits of the last
+        n_new nodes: the tree so far is ids with parents (index in the tree, -1
+        the root) and depths (the root's is 0); the nodes before the last n_new
+        are in the cache already, the new ones are appended, rotated to position
+        tokens before the tree + depth (KVCache.Rotate), and attended with
+        KVCache.AttendTree;
+      keep_path(n_nodes, path): KVCache.KeepPath on the model's sequence;
+      reset(): empty the cache.
+    widths: nodes of each level below the root; each is shared out over the level
+    above in order of the parents' probability under the draft.  Both caches hold
+    the committed tokens but the newest, which is the root of the next tree.  Of
+    `sampling` the temperature counts."""
+
+    def __init__(self, draft, target, widths=(4, 4, 4, 2), branch=2, sampling=None):
+        if not widths or min(widths) < 1 or branch < 1 or 1 + sum(widths) > MAX_TREE_NODES:
+            raise ValueError(f"levels of {tuple(widths)} nodes, {branch} a parent: at most {MAX_TREE_NODES} nodes")
+        self.draft, self.target = draft, target
+        self.widths, self.branch = tuple(widths), branch
+        self.sampling = sampling if sampling is not None else Sampler()
+
+    def _grow(self, root, levels):
+        """Draws a tree below `root` with the draft: ids, parents, depths and the
+        nodes' draft logits."""
+        temp = self.sampling.Temperature if self.sampling.Temperature > 0 else 1e-5
+        ids, parents, depths = [root], [-1], [0]
+        rows = [self.draft.forward_tree(ids, parents, depths, 1)]
+        score, level = {0: 0.0}, [0]
+        for width in levels:
+            order = sorted(level, key=lambda j: -score[j])
+            fresh = []
+            for rank, j in enumerate(order):
+                take = min(self.branch, width - len(fresh), rows[0].shape[1])
+                if take <= 0:
+                    break
+                logp = torch.log_softmax(torch.cat(rows)[j].double() / temp, dim=0)
+                # without replacement, in order: the largest of logits plus Gumbel noise
+                u = torch.from_numpy(self.sampling.Rand.take(logp.numel())).to(logp.device).double()
+                best = torch.topk(logp - torch.log(-torch.log(u.clamp(1e-12, 1 - 1e-9))), take)
+                for x in best.indices.tolist():
+                    if logp[x] == -float("inf"):
+                        continue
+                    score[len(ids)] = score[j] + float(logp[x])
+                    fresh.append(len(ids))
+                    ids.append(x)
+                    parents.append(j)
+                    depths.append(depths[j] + 1)
+            if not fresh:
+                break
+            rows.append(self.draft.forward_tree(ids, parents, depths, len(fresh)))
+            level = fresh
+        return ids, parents, depths, torch.cat(rows)
+
+    def Generate(self, prompt, max_new):
+        if not prompt:
+            raise ValueError("speculative: empty prompt")
+        d, t, smp = self.draft, self.target, self.sampling
+        d.reset()
+        t.reset()
+        if len(prompt) > 1:
+            d.forward(list(prompt[:-1]))
+            t.forward(list(prompt[:-1]))
+        root, gen = prompt[-1], []
+        drafted = accepted = 0
+        while len(gen) < max_new:
+            ids, parents, depths, q = self._grow(root, self.widths[:max_new - len(gen)])
+            p = t.forward_tree(ids, parents, depths, len(ids))
+            dev = p.device
+            u = torch.from_numpy(smp.Rand.take(len(ids))).to(dev)
+            paths, nxt = tree_accept(t.cache, p, torch.tensor(ids, dtype=torch.int32, device=dev),
+                                     torch.tensor(parents, dtype=torch.int32, device=dev), [len(ids)], u, smp,
+                                     draft_logits=q)
+            d.keep_path(len(ids), paths[0])
+            t.keep_path(len(ids), paths[0])
+            gen += [ids[j] for j in paths[0][1:]] + [nxt[0]]
+            root = nxt[0]
+            drafted += len(ids) - 1
+            accepted += len(paths[0]) - 1
         return gen[:max_new], (accepted / drafted if drafted else 0.0)
