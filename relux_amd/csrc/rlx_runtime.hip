@@ -3288,19 +3288,38 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
         node0 += n_nodes[i];
     }
     const std::vector<int> cuts = tree_cuts(load, c->kvh, c->cus, qt, c->hd, fine);
-    int64_t wgs = 0, parts = 0;
+    int64_t wgs = 0, parts = 0, n_cuts = 0;
+    int max_tiles = 1;
     bool merge = false;
+    // the longest cuts first, so that the last round is of short ones
+    std::vector<int> order(n_seqs);
     for (int i = 0; i < n_seqs; i++) {
+        order[i] = i;
+        n_cuts += cuts[i];
+        max_tiles = std::max(max_tiles, load[i].tiles);
+    }
+    std::stable_sort(order.begin(), order.end(), [&](int x, int y) {
+        return (int64_t)load[x].len * cuts[y] > (int64_t)load[y].len * cuts[x];
+    });
+    const bool spread = n_cuts >= 16;
+    std::vector<TreeRow> by_cut(n_seqs);
+    int at = 0;
+    for (int k = 0; k < n_seqs; k++) {
+        const int i = order[k];
         const int64_t n = (int64_t)load[i].tiles * c->kvh * cuts[i];
-        rows[i].nsplit = cuts[i];
-        rows[i].wg0 = (int32_t)wgs;
-        rows[i].part = (int32_t)parts;
+        by_cut[k] = rows[i];
+        by_cut[k].nsplit = cuts[i];
+        by_cut[k].at0 = spread ? at : (int32_t)wgs;
+        by_cut[k].part = (int32_t)parts;
+        at += cuts[i];
         wgs += n;
         if (cuts[i] > 1) {
             parts += n;
             merge = true;
         }
     }
+    rows.swap(by_cut);
+    if (spread) wgs = (n_cuts + 7) / 8 * 8 * c->kvh * max_tiles;
     if (wgs > 0x7FFFFFFF) return fail(RLX_ERR_UNSUPPORTED, "rlx_gqa_attend_tree: %lld work-groups", (long long)wgs);
     int32_t rc;
     if ((rc = flush_patches(c))) return rc;
@@ -3311,9 +3330,11 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
     if (rows.size() * sizeof(TreeRow) <= sizeof plan) {
         memcpy(plan.b, rows.data(), rows.size() * sizeof(TreeRow));
     } else {
-        std::vector<int32_t> work((size_t)wgs);
-        for (int i = 0, w = 0; i < n_seqs; i++)
-            for (int k = load[i].tiles * c->kvh * cuts[i]; k > 0; k--) work[w++] = i;
+        std::vector<int32_t> work;
+        for (int k = 0; k < n_seqs; k++) {
+            const int i = order[k];
+            work.insert(work.end(), spread ? cuts[i] : load[i].tiles * c->kvh * cuts[i], k);
+        }
         Blob b;
         const size_t o_r = b.add(rows), o_w = b.add(work);
         void *dev;
@@ -3338,6 +3359,9 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
     a.q_bf16 = q_dtype == RLX_BF16;
     a.out_bf16 = out_dtype == RLX_BF16;
     a.layout = qo_layout;
+    a.spread = spread;
+    a.n_at = (int)n_cuts;
+    a.max_tiles = max_tiles;
     if (!(scale > 0.f)) scale = (float)(1.0 / std::sqrt((double)c->hdu));
     a.qscale = scale * 1.4426950408889634f;
     hipEvent_t e0, e1;

@@ -25,14 +25,6 @@ __device__ __forceinline__ TreeRow tree_row(const TreeRow *rows, int i) {
     return TreeRow{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]};
 }
 
-// Place of (stream, tile) among a row's work-groups.  A stream is one kv head's
-// keys of one cut; its tiles read the same keys, so they stand 8 apart: the
-// same XCD (work-group b runs on XCD b mod 8), at about the same time.
-__device__ __forceinline__ int tree_place(int stream, int tile, int streams, int tiles) {
-    const int s0 = stream & ~7, m = min(8, streams - s0);
-    return s0 * tiles + tile * m + (stream - s0);
-}
-
 __device__ __forceinline__ void tree_store4(void *out, int64_t o, const float (&v)[4], int out_bf16) {
     if (out_bf16) {
         uint16_t *dst = (uint16_t *)out + o;
@@ -94,220 +86,201 @@ __device__ __forceinline__ void tree_ancestors(const int32_t *parents, int n, ui
     }
 }
 
-// Work-group = (cut of the keys, kv head, tile of query rows): 4 waves, each
-// holding all of the tile's 16 NQT query rows and taking every fourth unit of 32
-// keys, straight from HBM (or L2) into registers in the operand order of the
-// matrix instructions -- no LDS and no barrier in the loop:
+// What a work-group computes: a cut of one kv head's keys for a tile of query rows.
+struct TreeItem {
+    TreeRow R;
+    int nodes, nq, G, QR, tiles, split, kvh, tile, ctx, u0, u1;  // ctx: first key of the tree; u: units of 32 keys
+};
+// The item of work-group blockIdx.x; false: none.
 //
-//   S^T[32 keys][16 rows] = K[32 x D] . Q^T         2 D/32 MFMA 16x16x32 a tile
-//   P = exp2(S c - m), lane-local
-//   O^T[D][16 rows]      += V^T[D x 32 keys] . P^T  D/16 MFMA 16x16x32 a tile
-//
-// The 32 keys are two 16-token blocks of the pages; the order in which the
-// second product sums them is free, so a lane's 4 + 4 scores of the blocks are
-// its 8 operands as they are.
-//
-// The maximum of a row moves only when a score exceeds it by 2^8 (weights stay
-// below 256 in f32 and bf16 alike), so that rescaling and the reduction over
-// lanes are rare.
-//
-// Weights are rounded to bf16 for the second product, and the sum is of the
-// rounded ones.  FINE (f32 queries or outputs): queries in three bf16 parts
-// (exact), weights in two (2^-17).
-//
-// A masked weight is a selected zero; a value that is not finite in a masked
-// place must not reach other rows through 0 x inf, so such values of the tree's
-// keys stay out of the product and are added at the end to the rows that attend
-// them (an infinity or NaN whatever its weight).
-template <int D, int NQT, bool FINE>
-__global__ __launch_bounds__(256, 1) void tree_attend_kernel(PlanArg plan, TreeArgs a) {
-    constexpr int KS = D < 32 ? 1 : D / 32;
-    constexpr int MT = D / 16;
-    constexpr int QP = FINE ? 3 : 1;  // bf16 parts of a query
-    constexpr int QT = 16 * NQT;
-    const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-
-    __shared__ uint32_t anc[kTreeMaxNodes / 32][kTreeMaxNodes];
-    __shared__ int16_t up[kTreeMaxNodes];
-    __shared__ float sm[4][QT], sl[4][QT];
-    constexpr int MC = MT < 8 ? MT : 8;  // m-tiles merged at a time
-    __shared__ fl4 so[4][MC][64];
-
+// Work-group b runs on XCD b mod 8, each with its own L2 and address translation.
+// With cuts enough (a.spread) the cuts of all sequences, end to end, are dealt
+// out over the XCDs and a cut's kv heads and tiles run on one: they read the same
+// pages, 4 KB apart, and tiles the same keys.  The 16 x 8192 token call: .... With
+// few cuts that would leave XCDs idle: a row's cuts and kv heads are dealt out, a
+// pair's tiles 8 apart.
+template <int QT>
+__device__ __forceinline__ bool tree_item(const TreeArgs &a, TreeItem &w) {
     const int b = blockIdx.x;
+    int at = b, i = 0;  // what the rows are searched by; the item within a cut
+    if (a.spread) {
+        const int per = a.KVH * a.max_tiles, y = b >> 3;
+        at = y / per * 8 + (b & 7);
+        i = y % per;
+        if (at >= a.n_at) return false;
+    }
     int r;
     if (a.rows) {
-        r = ((kconst_i32 *)(uintptr_t)a.work)[b];
+        r = ((kconst_i32 *)(uintptr_t)a.work)[at];
     } else {
         int lo = 0, hi = a.n_rows - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (plan_ints(nullptr, mid, 8)[6] <= b)
+            if (plan_ints(nullptr, mid, 8)[6] <= at)
                 lo = mid;
             else
                 hi = mid - 1;
         }
         r = lo;
     }
-    const TreeRow R = tree_row(a.rows, r);
-    const int nodes = R.nodes & 0xFFFF, nq = R.nodes >> 16;
-    const int KVH = a.KVH, G = a.H / KVH, QR = nq * G;
-    const int tiles = (QR + QT - 1) / QT, streams = R.nsplit * KVH;
-    int tile, stream;
-    {
-        const int i = b - R.wg0, s0 = i / (8 * tiles) * 8, m = min(8, streams - s0), rem = i - s0 * tiles;
-        tile = rem / m;
-        stream = s0 + rem - tile * m;
+    w.R = tree_row(a.rows, r);
+    w.nodes = w.R.nodes & 0xFFFF;
+    w.nq = w.R.nodes >> 16;
+    w.G = a.H / a.KVH;
+    w.QR = w.nq * w.G;
+    w.tiles = (w.QR + QT - 1) / QT;
+    if (a.spread) {
+        w.split = at - w.R.at0;
+        w.kvh = i / a.max_tiles;
+        w.tile = i - w.kvh * a.max_tiles;
+        if (w.tile >= w.tiles) return false;
+    } else {
+        const int streams = w.R.nsplit * a.KVH;
+        i = b - w.R.at0;
+        const int s0 = i / (8 * w.tiles) * 8, m = min(8, streams - s0), rem = i - s0 * w.tiles;
+        w.tile = rem / m;
+        const int stream = s0 + rem - w.tile * m;
+        w.split = stream / a.KVH;
+        w.kvh = stream - w.split * a.KVH;
     }
-    const int split = stream / KVH, kvh = stream - split * KVH;
-    const int len = R.len, ctx = len - nodes;  // first key of the tree
-    const int units = (len + kTreeKeys - 1) / kTreeKeys;
-    const int u0 = (int)((int64_t)split * units / R.nsplit), u1 = (int)((int64_t)(split + 1) * units / R.nsplit);
-    const bool has_tree = u1 * kTreeKeys > ctx;
-    if (has_tree) tree_ancestors(a.parents + R.node0, nodes, anc, up);
+    w.ctx = w.R.len - w.nodes;
+    const int units = (w.R.len + kTreeKeys - 1) / kTreeKeys;
+    w.u0 = (int)((int64_t)w.split * units / w.R.nsplit);
+    w.u1 = (int)((int64_t)(w.split + 1) * units / w.R.nsplit);
+    return true;
+}
+// Partial slot of (cut, kv head, tile) of a row.
+__device__ __forceinline__ int64_t tree_slot(const TreeRow &R, int KVH, int tiles, int split, int kvh, int tile) {
+    return (int64_t)R.part + ((int64_t)split * KVH + kvh) * tiles + tile;
+}
 
-    // ---- this wave's units: u0 + wave, + 4, ... --------------------------------
-    const int first = u0 + wave, nu = first < u1 ? (u1 - first + 3) / 4 : 0;
-    // Pages and slots of 32 units' blocks, one block a lane.  A block past the
-    // last token reads the last token's (its keys are masked).
-    int pg = 0, sl0 = 0;
-    auto fetch_pages = [&](int j0) {
-        const int j = j0 + (lane >> 1);
-        int t = (first + 4 * min(j, nu - 1)) * kTreeKeys + 16 * (lane & 1);
-        t = min(t, (len - 1) & ~15);
-        const int e = a.pshift >= 0 ? t >> a.pshift : t / a.P;
-        pg = a.table[R.tab + e];
-        sl0 = t - e * a.P;
-    };
-    if (nu > 0) fetch_pages(0);
-    asm volatile("" ::"v"(pg), "v"(sl0));
-
-    // ---- queries: B operand, lane (row col, dims grp * 8 ..) -------------------
-    u32x4 qb[NQT][KS][QP];
-    int node[NQT];  // the row's node; rows past the tile's hold zeros
+// The bf16 parts (the high one, or three whose sum is the f32 value) of 8 values.
+template <int PARTS>
+__device__ __forceinline__ void tree_parts(float (&v)[8], u32x4 (&o)[PARTS]) {
 #pragma unroll
-    for (int nt = 0; nt < NQT; nt++) {
-        const int qr = tile * QT + nt * 16 + col;
-        const bool ok = qr < QR;
-        const int qc = ok ? qr : 0;
-        node[nt] = nodes - nq + qc / G;
-        const int64_t base = tree_qbase(a, R, kvh, G, qc);
+    for (int p = 0; p < PARTS; p++)
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const int d0 = ks * 32 + grp * 8;
-            const bool in = ok && d0 < a.DQ;
-            float v[8];
-            if (a.q_bf16) {
-                const u32x4 w = in ? *(const u32x4 *)((const uint16_t *)a.q + base + d0) : u32x4{0, 0, 0, 0};
-                qb[nt][ks][0] = w;
-                if constexpr (FINE) qb[nt][ks][1] = qb[nt][ks][2] = u32x4{0, 0, 0, 0};
-                continue;
-            }
-            const float4 x = in ? *(const float4 *)((const float *)a.q + base + d0) : float4{0.f, 0.f, 0.f, 0.f};
-            const float4 y = in ? *(const float4 *)((const float *)a.q + base + d0 + 4) : float4{0.f, 0.f, 0.f, 0.f};
-            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-#pragma unroll
-            for (int p = 0; p < QP; p++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint16_t h0 = bf16_rne(v[2 * i]), h1 = bf16_rne(v[2 * i + 1]);
-                    qb[nt][ks][p][i] = (uint32_t)h0 | ((uint32_t)h1 << 16);
-                    v[2 * i] -= bf16_f32(h0);
-                    v[2 * i + 1] -= bf16_f32(h1);
-                }
+        for (int i = 0; i < 4; i++) {
+            o[p][i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+            v[2 * i] -= bf16_lo(o[p][i]);
+            v[2 * i + 1] -= bf16_hi(o[p][i]);
         }
-    }
+}
 
+// A wave's 16 NQT query rows and their running softmax over units of 32 keys:
+//
+//   S^T[32 keys][16 rows] = K[32 x D] . Q^T         2 D/32 MFMA 16x16x32 a tile
+//   P = exp2(S c - m), lane-local
+//   O^T[D][16 rows]      += V^T[D x 32 keys] . P^T  D/16 MFMA 16x16x32 a tile
+//
+// Rows of the two 16-key score tiles are given the keys 8 (row / 4) + row % 4 and
+// 4 more, so that a lane's scores are those of 8 consecutive keys: the operand of
+// the second product as they are, against V read 8 keys (16 bytes) at a time.
+//
+// The maximum of a row moves only when a score exceeds it by 2^8 (weights stay
+// below 256 in f32 and bf16 alike), so that rescaling and the reduction over
+// lanes are rare.
+//
+// Weights are rounded to bf16 for the second product, and the sum is of the
+// rounded ones.  FINE (f32 queries or outputs): queries and weights in three
+// bf16 parts, as exact as f32.
+//
+// A masked weight is a selected zero; a value that is not finite in a masked
+// place must not reach other rows through 0 x inf, so such values of the tree's
+// keys stay out of the product and are added at the end to the rows that attend
+// them (an infinity or NaN whatever its weight).
+template <int D, int NQT, bool FINE, bool ACC>
+struct TreeWave {
+    static constexpr int KS = D < 32 ? 1 : D / 32, MT = D / 16, PARTS = FINE ? 3 : 1;
+    u32x4 qb[NQT][KS][PARTS];
+    int node[NQT];
     float m_run[NQT], l_part[NQT];
     fl4 acc[NQT][MT];
+    bool odd = false;  // a value of the tree's keys that is not finite
+    int col, grp, len, ctx;
+    const uint32_t (*anc)[kTreeMaxNodes];
+
+    // Query rows row0 + 16 nt + col; rows past the last one hold zeros.
+    __device__ __forceinline__ void init(const TreeArgs &a, const TreeItem &w, int row0, const uint32_t (*an)[kTreeMaxNodes]) {
+        const int lane = threadIdx.x & 63;
+        col = lane & 15;
+        grp = lane >> 4;
+        len = w.R.len;
+        ctx = w.ctx;
+        anc = an;
 #pragma unroll
-    for (int nt = 0; nt < NQT; nt++) {
-        m_run[nt] = -INFINITY;
-        l_part[nt] = 0.f;
+        for (int nt = 0; nt < NQT; nt++) {
+            const int qr = row0 + nt * 16 + col;
+            const bool ok = qr < w.QR;
+            const int qc = ok ? qr : 0;
+            node[nt] = w.nodes - w.nq + qc / w.G;
+            const int64_t base = tree_qbase(a, w.R, w.kvh, w.G, qc);
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) acc[nt][mt] = fl4{0.f, 0.f, 0.f, 0.f};
+            for (int ks = 0; ks < KS; ks++) {
+                const int d0 = ks * 32 + grp * 8;
+                const bool in = ok && d0 < a.DQ;
+                if (a.q_bf16) {
+                    qb[nt][ks][0] = in ? *(const u32x4 *)((const uint16_t *)a.q + base + d0) : u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int p = 1; p < PARTS; p++) qb[nt][ks][p] = u32x4{0, 0, 0, 0};
+                } else {
+                    const float4 z = float4{0.f, 0.f, 0.f, 0.f};
+                    const float4 x = in ? *(const float4 *)((const float *)a.q + base + d0) : z;
+                    const float4 y = in ? *(const float4 *)((const float *)a.q + base + d0 + 4) : z;
+                    float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                    tree_parts<PARTS>(v, qb[nt][ks]);
+                }
+            }
+            m_run[nt] = -INFINITY;
+            l_part[nt] = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) acc[nt][mt] = fl4{0.f, 0.f, 0.f, 0.f};
+        }
     }
 
-    const int64_t head = (int64_t)a.P * D;  // one kv head of one page
-    const uint32_t k_lane = (D == 16 ? col * 16 + (grp & 1) * 8 : col * 32 + grp * 8) * 2u;  // bytes
-    uint32_t v_lane[MT];
+    // The queries are here: no wait for them sits in the loop, where it would
+    // wait for the keys requested ahead as well.
+    __device__ __forceinline__ void ready() const {
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) v_lane[mt] = (uint32_t)((mt * 16 + col) * a.P + grp * 4) * 2u;
-    auto load_unit = [&](int j, u32x4(&kr)[2][KS], u32x4(&vr)[MT]) {
-        j = min(j, nu - 1);
-        if ((j & 31) == 0 && j) {
-            fetch_pages(j);
-            asm volatile("" ::"v"(pg), "v"(sl0));
-        }
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int src = (2 * j + k) & 63;
-            const int page = __builtin_amdgcn_readlane(pg, src), slot = __builtin_amdgcn_readlane(sl0, src);
-            const int64_t base = ((int64_t)page * KVH + kvh) * head;
-            const char *kp = (const char *)(a.kpool + base + (int64_t)slot * D);
-            const char *vp = (const char *)(a.vpool + base + slot);
+        for (int nt = 0; nt < NQT; nt++)
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
-                kr[k][ks] = __builtin_nontemporal_load((const u32x4 *)(kp + (k_lane + ks * 1024)));
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                const u32x2 w = __builtin_nontemporal_load((const u32x2 *)(vp + v_lane[mt]));
-                vr[mt][2 * k] = w[0];
-                vr[mt][2 * k + 1] = w[1];
-            }
-        }
-    };
+                for (int p = 0; p < PARTS; p++) asm volatile("" ::"v"(qb[nt][ks][p]));
+    }
 
-    // Key i of block k in a lane: t0 + 16 k + 4 grp + i.
-    auto allowed = [&](int t, int nt) {
+    __device__ __forceinline__ bool allowed(int t, int nt) const {
         if (t < ctx) return true;
         const int k = t - ctx;
         return t < len && ((anc[k >> 5][node[nt]] >> (k & 31)) & 1u);
-    };
+    }
 
-    bool odd = false;  // a value of the tree's keys that is not finite
-    // tree: a unit that holds keys of the tree (or past the last token)
-    auto consume = [&](auto tree, int j, u32x4(&kr)[2][KS], u32x4(&vr)[MT]) {
-        constexpr bool TREE = decltype(tree)::value;
-        const int t0 = (first + 4 * j) * kTreeKeys;
-        if constexpr (TREE) {
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int t = t0 + 16 * k + 4 * grp + i;
-                    const uint32_t keep = (i & 1) ? 0x0000FFFFu : 0xFFFF0000u;
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        const uint32_t w = vr[mt][2 * k + (i >> 1)] & ~keep, ex = 0x7F807F80u & ~keep;
-                        const bool inf = t >= ctx && (w & ex) == ex;
-                        odd |= inf && t < len;
-                        if (t >= len || inf) vr[mt][2 * k + (i >> 1)] &= keep;
-                    }
-                }
-        }
-        if (D == 16) {
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-                if (grp >= 2) kr[k][0] = u32x4{0, 0, 0, 0};
-        }
-        fl4 s[NQT][2];
+    typedef fl4 Scores[NQT][2];
+    typedef u32x4 Weights[NQT][PARTS];
+
+    // Scores of a unit; kf(k, ks): the keys' fragments.
+    template <class KF>
+    __device__ __forceinline__ void scores(Scores &s, KF kf) {
 #pragma unroll
         for (int nt = 0; nt < NQT; nt++) s[nt][0] = s[nt][1] = fl4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-            for (int p = QP - 1; p >= 0; p--)
+            for (int k = 0; k < 2; k++) {
+                const bf16x8 kr = __builtin_bit_cast(bf16x8, kf(k, ks));
 #pragma unroll
-                for (int nt = 0; nt < NQT; nt++)
+                for (int p = PARTS - 1; p >= 0; p--)
 #pragma unroll
-                    for (int k = 0; k < 2; k++)
-                        s[nt][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[k][ks]),
-                                                                          __builtin_bit_cast(bf16x8, qb[nt][ks][p]),
+                    for (int nt = 0; nt < NQT; nt++)
+                        s[nt][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr, __builtin_bit_cast(bf16x8, qb[nt][ks][p]),
                                                                           s[nt][k], 0, 0, 0);
+            }
+    }
+    // FINE: an infinite key against a query's parts of both signs is a NaN; its
+    // score is the first part's.
+    template <class KF>
+    __device__ __forceinline__ void mend(Scores &s, KF kf) {
         if constexpr (FINE) {
-            // An infinite key against a query's parts of both signs is a NaN; its
-            // score is the first part's.
             float sum = 0.f;
 #pragma unroll
             for (int nt = 0; nt < NQT; nt++)
@@ -315,100 +288,247 @@ __global__ __launch_bounds__(256, 1) void tree_attend_kernel(PlanArg plan, TreeA
                 for (int i = 0; i < 8; i++) sum += s[nt][i >> 2][i & 3];
             if (__builtin_amdgcn_ballot_w64(sum != sum)) {
 #pragma unroll
-                for (int nt = 0; nt < NQT; nt++)
+                for (int k = 0; k < 2; k++) {
+                    fl4 h[NQT];
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        fl4 h = fl4{0.f, 0.f, 0.f, 0.f};
+                    for (int nt = 0; nt < NQT; nt++) h[nt] = fl4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int ks = 0; ks < KS; ks++)
-                            h = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kr[k][ks]),
-                                                                        __builtin_bit_cast(bf16x8, qb[nt][ks][0]), h,
-                                                                        0, 0, 0);
+                    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                        for (int nt = 0; nt < NQT; nt++)
+                            h[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kf(k, ks)),
+                                                                            __builtin_bit_cast(bf16x8, qb[nt][ks][0]),
+                                                                            h[nt], 0, 0, 0);
+#pragma unroll
+                    for (int nt = 0; nt < NQT; nt++)
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            if (s[nt][k][i] != s[nt][k][i]) s[nt][k][i] = h[i];
-                    }
+                            if (s[nt][k][i] != s[nt][k][i]) s[nt][k][i] = h[nt][i];
+                }
             }
         }
-        if constexpr (TREE) {
+    }
+    // Masks a unit from key t0 that holds keys of the tree, or past the last token.
+    __device__ __forceinline__ void mask(Scores &s, int t0) const {
 #pragma unroll
-            for (int nt = 0; nt < NQT; nt++)
+        for (int nt = 0; nt < NQT; nt++)
 #pragma unroll
-                for (int k = 0; k < 2; k++)
+            for (int i = 0; i < 8; i++)
+                if (!allowed(t0 + grp * 8 + i, nt)) s[nt][i >> 2][i & 3] = -INFINITY;
+    }
+    // A lane's largest scores.
+    __device__ __forceinline__ void largest(const Scores &s, float (&mx)[NQT]) const {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (!allowed(t0 + 16 * k + 4 * grp + i, nt)) s[nt][k][i] = -INFINITY;
-        }
-        float mx[NQT];
-        bool grow = false;
+        for (int nt = 0; nt < NQT; nt++)
+            mx[nt] = max3(max3(max3(s[nt][0][0], s[nt][0][1], s[nt][0][2]), s[nt][0][3], s[nt][1][0]), s[nt][1][1],
+                          max3(s[nt][1][2], s[nt][1][3], s[nt][1][3]));
+    }
+    // (as one instruction: fmaxf makes its operands canonical first)
+    static __device__ __forceinline__ float max3(float x, float y, float z) {
+        float r;
+        asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+        return r;
+    }
+    // Moves the maximum (and what was summed under it) where a score exceeds it far.
+    __device__ __forceinline__ void grow(const float (&mx)[NQT], float qscale) {
+        bool far = false;
+#pragma unroll
+        for (int nt = 0; nt < NQT; nt++) far |= mx[nt] * qscale > m_run[nt] + 8.f;
+        if (!__builtin_amdgcn_ballot_w64(far)) return;
 #pragma unroll
         for (int nt = 0; nt < NQT; nt++) {
-            mx[nt] = fmaxf(fmaxf(fmaxf(s[nt][0][0], s[nt][0][1]), fmaxf(s[nt][0][2], s[nt][0][3])),
-                           fmaxf(fmaxf(s[nt][1][0], s[nt][1][1]), fmaxf(s[nt][1][2], s[nt][1][3])));
-            grow |= mx[nt] * a.qscale > m_run[nt] + 8.f;
-        }
-        if (__builtin_amdgcn_ballot_w64(grow)) {
+            const float m_new = fmaxf(m_run[nt], rows4_max(mx[nt]) * qscale);
+            const float c = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[nt] - m_new);
+            m_run[nt] = m_new;
+            l_part[nt] *= c;
 #pragma unroll
-            for (int nt = 0; nt < NQT; nt++) {
-                const float m_new = fmaxf(m_run[nt], rows4_max(mx[nt]) * a.qscale);
-                const float c = m_new == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_run[nt] - m_new);
-                m_run[nt] = m_new;
-                l_part[nt] *= c;
-#pragma unroll
-                for (int mt = 0; mt < MT; mt++) acc[nt][mt] *= c;
+            for (int mt = 0; mt < MT; mt++) {
+                // (pinned on both sides, so that the loop does not carry copies
+                // for this branch)
+                pin(acc[nt][mt]);
+                acc[nt][mt] *= c;
+                pin(acc[nt][mt]);
             }
         }
+    }
+    // Accumulators live in accumulation registers where a wave has more than 256.
+    static __device__ __forceinline__ void pin(fl4 &x) {
+        if constexpr (ACC)
+            asm volatile("" : "+a"(x));
+        else
+            asm volatile("" : "+v"(x));
+    }
+    __device__ __forceinline__ void weights(const Scores &s, Weights &pw, float qscale) {
 #pragma unroll
         for (int nt = 0; nt < NQT; nt++) {
             const float m = m_run[nt] == -INFINITY ? 0.f : m_run[nt];
-            u32x4 pw, pl;
             float p[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[nt][i >> 2][i & 3], a.qscale, -m));
+            for (int i = 0; i < 8; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[nt][i >> 2][i & 3], qscale, -m));
+            if constexpr (FINE) l_part[nt] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            tree_parts<PARTS>(p, pw[nt]);
+            if constexpr (!FINE)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                pw[i] = pack_bf16x2(p[2 * i], p[2 * i + 1]);
-                if constexpr (FINE) {
-                    pl[i] = pack_bf16x2(p[2 * i] - bf16_lo(pw[i]), p[2 * i + 1] - bf16_hi(pw[i]));
-                    l_part[nt] += p[2 * i] + p[2 * i + 1];
-                } else {
-                    l_part[nt] = add_bf16x2(pw[i], l_part[nt]);
+                for (int i = 0; i < 4; i++) l_part[nt] = add_bf16x2(pw[nt][0][i], l_part[nt]);
+        }
+    }
+    // The values' product; vf(mt): their fragments.  TREE: as mask().
+    template <bool TREE, class VF>
+    __device__ __forceinline__ void values(const Weights &pw, int t0, VF vf) {
+        const int tl = t0 + grp * 8;
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            u32x4 v = vf(mt);
+            if constexpr (TREE) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t keep = (i & 1) ? 0x0000FFFFu : 0xFFFF0000u, ex = 0x7F807F80u & ~keep;
+                    const bool inf = tl + i >= ctx && (v[i >> 1] & ex) == ex;
+                    odd |= inf && tl + i < len;
+                    if (tl + i >= len || inf) v[i >> 1] &= keep;
                 }
             }
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                if constexpr (FINE)
+            for (int p = PARTS - 1; p >= 0; p--)
+#pragma unroll
+                for (int nt = 0; nt < NQT; nt++)
                     acc[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, vr[mt]), __builtin_bit_cast(bf16x8, pl), acc[nt][mt], 0, 0, 0);
-                acc[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                    __builtin_bit_cast(bf16x8, vr[mt]), __builtin_bit_cast(bf16x8, pw), acc[nt][mt], 0, 0, 0);
+                        __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pw[nt][p]), acc[nt][mt], 0, 0, 0);
+        }
+    }
+
+    // The tree's values that are not finite, for dims d0 .. d0 + 3 of row tile nt.
+    __device__ __forceinline__ void add_odd(const TreeArgs &a, const TreeItem &w, int nt, int d0, fl4 &o) const {
+#pragma unroll 1
+        for (int t = max(w.u0 * kTreeKeys, ctx); t < min(w.u1 * kTreeKeys, len); t++) {
+            if (!allowed(t, nt)) continue;
+            const int e = t / a.P;
+            const uint16_t *vp = a.vpool + ((int64_t)a.table[w.R.tab + e] * a.KVH + w.kvh) * a.P * D + (t - e * a.P);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint16_t x = vp[(d0 + i) * a.P];
+                if ((x & 0x7F80) == 0x7F80) o[i] += bf16_f32(x);
             }
         }
+    }
+};
+
+// Byte offsets into the K and V pools of a lane's block (lane & 1) of unit j +
+// lane / 2, of `nu` units `step` apart from unit `first`.  A block past the last
+// token is the last token's (its keys are masked).
+template <int D>
+struct TreePages {
+    int64_t k, v;
+    __device__ __forceinline__ void fetch(const TreeArgs &a, const TreeItem &w, int first, int step, int nu, int j) {
+        const int lane = threadIdx.x & 63;
+        int t = (first + step * min(j + (lane >> 1), nu - 1)) * kTreeKeys + 16 * (lane & 1);
+        t = min(t, (w.R.len - 1) & ~15);
+        const int e = a.pshift >= 0 ? t >> a.pshift : t / a.P, slot = t - e * a.P;
+        const int64_t base = ((int64_t)a.table[w.R.tab + e] * a.KVH + w.kvh) * a.P * D;
+        k = (base + (int64_t)slot * D) * 2;
+        v = (base + slot) * 2;
+        // wait here, so that no wait for these sits on the common path
+        asm volatile("" ::"v"(k), "v"(v));
+    }
+    // A lane's offset in unit j of the fetched ones: that of its block.
+    static __device__ __forceinline__ int64_t pick(int64_t off, int j, bool second) {
+        const int src = (2 * j) & 63;
+        const auto at = [&](int l) {
+            const uint32_t lo = __builtin_amdgcn_readlane((int)off, l), hi = __builtin_amdgcn_readlane((int)(off >> 32), l);
+            return (int64_t)((uint64_t)hi << 32 | lo);
+        };
+        const int64_t x = at(src), y = at(src + 1);
+        return second ? y : x;
+    }
+};
+// A lane's places in a unit: K of key 8 (col / 4) + col % 4 (kKeys4 bytes on: the
+// second score tile's, 4 keys further; kStep: the next 32 dims), dims 8 grp ..;
+// V of dim col, keys 8 grp ...
+template <int D>
+struct TreeLane {
+    static constexpr int kKeys4 = D <= 32 ? 4 * D * 2 : 256, kStep = 1024;
+    const char *k, *v;
+    bool k2, v2;  // in the unit's second block
+    __device__ __forceinline__ explicit TreeLane(const TreeArgs &a) {
+        const int lane = threadIdx.x & 63, col = lane & 15, grp = lane >> 4, row = ((col >> 2) & 1) * 8 + (col & 3);
+        k = (const char *)a.kpool + (D == 16 ? row * 32 + (grp & 1) * 16 : row * 64 + grp * 16);
+        v = (const char *)a.vpool + (col * a.P + (grp & 1) * 8) * 2;
+        k2 = col >= 8;
+        v2 = grp >= 2;
+    }
+};
+
+// Few query rows: 4 waves, each holding all 16 NQT rows of the tile and taking
+// every fourth unit, straight from HBM into registers in the operands' order -- no
+// LDS and no barrier in the loop.  HBM-bound.
+template <int D, int NQT, bool FINE>
+__global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeArgs a) {
+    using W = TreeWave<D, NQT, FINE, true>;
+    constexpr int KS = W::KS, MT = W::MT, QT = 16 * NQT;
+    constexpr int MC = MT < 8 ? MT : 8;  // m-tiles merged at a time
+    __shared__ uint32_t anc[kTreeMaxNodes / 32][kTreeMaxNodes];
+    __shared__ int16_t up[kTreeMaxNodes];
+    __shared__ float sm[4][QT], sl[4][QT];
+    __shared__ fl4 so[4][MC][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TreeItem w;
+    if (!tree_item<QT>(a, w)) return;
+    if (w.u1 * kTreeKeys > w.ctx) tree_ancestors(a.parents + w.R.node0, w.nodes, anc, up);
+
+    const int first = w.u0 + wave, nu = first < w.u1 ? (w.u1 - first + 3) / 4 : 0;
+    const int nc = max(0, min(nu, (w.ctx / kTreeKeys - first + 3) / 4));  // units before the tree's
+    TreePages<D> pages;
+    if (nu > 0) pages.fetch(a, w, first, 4, nu, 0);
+    const TreeLane<D> at(a);
+    W q;
+    q.init(a, w, w.tile * QT, anc);
+
+    auto load = [&](int j, u32x4(&kr)[2][KS], u32x4(&vr)[MT]) {
+        j = min(j, nu - 1);
+        if ((j & 31) == 0 && j) pages.fetch(a, w, first, 4, nu, j);
+        const char *kp = at.k + pages.pick(pages.k, j, at.k2), *vp = at.v + pages.pick(pages.v, j, at.v2);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                kr[k][ks] = __builtin_nontemporal_load((const u32x4 *)(kp + ks * at.kStep + k * at.kKeys4));
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) vr[mt] = __builtin_nontemporal_load((const u32x4 *)(vp + mt * a.P * 32));
+    };
+    auto consume = [&](auto tree, int j, u32x4(&kr)[2][KS], u32x4(&vr)[MT]) {
+        constexpr bool TREE = decltype(tree)::value;
+        const int t0 = (first + 4 * j) * kTreeKeys;
+        const auto kf = [&](int k, int ks) { return D == 16 && q.grp >= 2 ? u32x4{0, 0, 0, 0} : kr[k][ks]; };
+        typename W::Scores sc;
+        typename W::Weights pw;
+        float mx[NQT];
+        q.scores(sc, kf);
+        q.mend(sc, kf);
+        if constexpr (TREE) q.mask(sc, t0);
+        q.largest(sc, mx);
+        q.grow(mx, a.qscale);
+        q.weights(sc, pw, a.qscale);
+        q.template values<TREE>(pw, t0, [&](int mt) { return vr[mt]; });
     };
     using Ctx = std::integral_constant<bool, false>;
     using Tree = std::integral_constant<bool, true>;
-
     // Two register sets alternate, so that the next unit's loads are in flight
     // while one is consumed (past the last unit they read it again).  Stored head
     // dim 256 has registers for one.
-    const int nc = max(0, min(nu, (ctx / kTreeKeys - first + 3) / 4));  // units before the tree's
-    u32x4 ka[2][KS], kb[2][KS];
-    u32x4 va[MT], vb[MT];
+    u32x4 ka[2][KS], kb[2][KS], va[MT], vb[MT];
     int j = 0;
     if constexpr (D <= 128) {
-        if (nu > 0) load_unit(0, ka, va);
+        if (nu > 0) load(0, ka, va);
+        q.ready();
         for (; j + 1 < nc; j += 2) {
-            load_unit(j + 1, kb, vb);
+            load(j + 1, kb, vb);
             consume(Ctx{}, j, ka, va);
-            load_unit(j + 2, ka, va);
+            load(j + 2, ka, va);
             consume(Ctx{}, j + 1, kb, vb);
         }
         for (; j < nu; j++) {
-            load_unit(j + 1, kb, vb);
-            if (j < nc)
-                consume(Ctx{}, j, ka, va);
-            else
-                consume(Tree{}, j, ka, va);
+            load(j + 1, kb, vb);
+            consume(Tree{}, j, ka, va);
 #pragma unroll
             for (int i = 0; i < KS; i++) ka[0][i] = kb[0][i], ka[1][i] = kb[1][i];
 #pragma unroll
@@ -416,69 +536,202 @@ __global__ __launch_bounds__(256, 1) void tree_attend_kernel(PlanArg plan, TreeA
         }
     } else {
         for (; j < nc; j++) {
-            load_unit(j, ka, va);
+            load(j, ka, va);
             consume(Ctx{}, j, ka, va);
         }
         for (; j < nu; j++) {
-            load_unit(j, ka, va);
+            load(j, ka, va);
             consume(Tree{}, j, ka, va);
         }
     }
 
-    // ---- merge of the 4 waves --------------------------------------------------
+    // ---- merge of the 4 waves ----
 #pragma unroll
     for (int nt = 0; nt < NQT; nt++) {
-        const float l = rows4_sum(l_part[nt]);
-        if (grp == 0) {
-            sm[wave][nt * 16 + col] = m_run[nt];
-            sl[wave][nt * 16 + col] = l;
+        const float l = rows4_sum(q.l_part[nt]);
+        if (q.grp == 0) {
+            sm[wave][nt * 16 + q.col] = q.m_run[nt];
+            sl[wave][nt * 16 + q.col] = l;
         }
     }
-    const bool any_odd = __syncthreads_or(odd);
-    const int slot = R.part + b - R.wg0;
+    const bool any_odd = __syncthreads_or(q.odd);
+    const int64_t slot = tree_slot(w.R, a.KVH, w.tiles, w.split, w.kvh, w.tile);
 #pragma unroll
     for (int nt = 0; nt < NQT; nt++) {
-        const int qt = nt * 16 + col, qr = tile * QT + qt;
+        const int qt = nt * 16 + q.col, qr = w.tile * QT + qt;
         float M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w][qt]);
+        for (int i = 0; i < 4; i++) M = fmaxf(M, sm[i][qt]);
 #pragma unroll
-        for (int w = 0; w < 4; w++) L += sm[w][qt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[w][qt] - M) * sl[w][qt];
-        const float f = m_run[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_run[nt] - M);
+        for (int i = 0; i < 4; i++) L += sm[i][qt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[i][qt] - M) * sl[i][qt];
+        const float f = q.m_run[nt] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(q.m_run[nt] - M);
         const float inv = L > 0.f ? 1.f / L : 0.f;
 #pragma unroll
         for (int m0 = 0; m0 < MT; m0 += MC) {
             if (nt || m0) __syncthreads();
 #pragma unroll
-            for (int mt = 0; mt < MC; mt++) so[wave][mt][lane] = acc[nt][m0 + mt] * f;
+            for (int mt = 0; mt < MC; mt++) so[wave][mt][lane] = q.acc[nt][m0 + mt] * f;
             __syncthreads();
             for (int mt = wave; mt < MC; mt += 4) {
                 fl4 o = (so[0][mt][lane] + so[1][mt][lane]) + (so[2][mt][lane] + so[3][mt][lane]);
-                const int d0 = (m0 + mt) * 16 + grp * 4;
-                if (any_odd) {
-#pragma unroll 1
-                    for (int t = max(u0 * kTreeKeys, ctx); t < min(u1 * kTreeKeys, len); t++) {
-                        if (!allowed(t, nt)) continue;
-                        const int e = t / a.P;
-                        const uint16_t *vp = a.vpool + ((int64_t)a.table[R.tab + e] * KVH + kvh) * head + (t - e * a.P);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint16_t w = vp[(d0 + i) * a.P];
-                            if ((w & 0x7F80) == 0x7F80) o[i] += bf16_f32(w);
-                        }
-                    }
-                }
-                if (R.nsplit > 1) {
-                    *(fl4 *)(a.part_o + ((int64_t)slot * QT + qt) * D + d0) = o;
-                } else if (qr < QR && d0 < a.DQ) {
+                const int d0 = (m0 + mt) * 16 + q.grp * 4;
+                if (any_odd) q.add_odd(a, w, nt, d0, o);
+                if (w.R.nsplit > 1) {
+                    *(fl4 *)(a.part_o + (slot * QT + qt) * D + d0) = o;
+                } else if (qr < w.QR && d0 < a.DQ) {
                     const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
-                    tree_store4(a.out, tree_qbase(a, R, kvh, G, qr) + d0, v, a.out_bf16);
+                    tree_store4(a.out, tree_qbase(a, w.R, w.kvh, w.G, qr) + d0, v, a.out_bf16);
                 }
             }
         }
-        if (R.nsplit > 1 && wave == 0 && grp == 0) {
-            float *pm = a.part_ml + ((int64_t)slot * QT + qt) * 2;
+        if (w.R.nsplit > 1 && wave == 0 && q.grp == 0) {
+            float *pm = a.part_ml + (slot * QT + qt) * 2;
             pm[0] = M;
+            pm[1] = L;
+        }
+    }
+}
+
+// Many query rows: WAVES waves of 16 NQT rows each share the keys, which stream
+// through a ring of units in LDS in the operands' order (a lane's 16 bytes of a
+// fragment at 16 lane: reads without bank conflicts).  A wave takes the scores of unit
+// u + 1 while it turns those of unit u into weights, so that the matrix unit works
+// through the softmax; two waves a SIMD hide the rest.  HBM-bound at few rows, by
+// the matrix and softmax units at many.
+template <int D, int NQT, int WAVES, bool FINE>
+__global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void tree_wide_kernel(PlanArg plan, TreeArgs a) {
+    using W = TreeWave<D, NQT, FINE, (D > 128 && WAVES == 4)>;
+    constexpr int KS = W::KS, MT = W::MT, QT = 16 * NQT * WAVES;
+    static_assert(D >= 64 && 2 * KS == MT, "K and V of a unit take as many loads");
+    constexpr int UNIT = 2 * MT * 64;                       // u32x4 of a unit: K, then V
+    constexpr int UPS = WAVES == 8 && D <= 128 ? 2 : 1;     // units a stage
+    constexpr int STAGES = 4;                               // of 16 KB a unit (D 128) or 32
+    constexpr int SLABS = UPS * 2 * MT, LOADS = (SLABS + WAVES - 1) / WAVES;  // fragments of a stage; a wave's of them
+    static_assert(SLABS % WAVES == 0 && MT % LOADS == 0, "a wave loads K or V");
+    __shared__ uint32_t anc[kTreeMaxNodes / 32][kTreeMaxNodes];
+    __shared__ int16_t up[kTreeMaxNodes];
+    __shared__ u32x4 ring[STAGES * UPS][UNIT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    TreeItem w;
+    if (!tree_item<QT>(a, w)) return;
+    if (w.u1 * kTreeKeys > w.ctx) tree_ancestors(a.parents + w.R.node0, w.nodes, anc, up);
+
+    const int nu = w.u1 - w.u0;
+    const int nc = max(0, min(nu, w.ctx / kTreeKeys - w.u0));  // units before the tree's
+    const bool shared = w.QR > QT;  // other tiles read the same keys
+    const uint32_t ring_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4 *)&ring[0][0];
+    TreePages<D> pages;
+    const TreeLane<D> at(a);
+    W q;
+    q.init(a, w, w.tile * QT + wave * 16 * NQT, anc);
+    q.ready();
+    const int ns = (nu + UPS - 1) / UPS;
+    // a wave's fragments are of one unit, and of K or V alone
+    const int i0 = wave * LOADS % (2 * MT), uu = wave * LOADS / (2 * MT);
+    const bool is_v = i0 >= MT;
+    auto issue = [&](int s) {
+        if ((s * UPS & 31) == 0) pages.fetch(a, w, w.u0, 1, nu, s * UPS);
+        const uint32_t dst = ring_lds + (uint32_t)(s % STAGES * UPS * UNIT + wave * LOADS * 64) * 16;
+        const char *src = is_v ? at.v + pages.pick(pages.v, s * UPS + uu, at.v2) + (i0 - MT) * a.P * 32
+                               : at.k + pages.pick(pages.k, s * UPS + uu, at.k2);
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) {
+            const int i = i0 + l;
+            const char *p = is_v ? src + l * a.P * 32 : src + (i >> 1) * at.kStep + (i & 1) * at.kKeys4;
+            if (shared)
+                lds_dma16_keep(p, dst + l * 1024);
+            else
+                lds_dma16(p, dst + l * 1024);
+        }
+    };
+    // Stage s is here: this wave's loads of it are done, then everybody's.  Stages
+    // up to s + STAGES - 3 were requested.
+    auto arrive = [&](int s) {
+        if (s + STAGES - 3 < ns)
+            RLX_WAIT_VM(LOADS * (STAGES - 3));
+        else
+            RLX_WAIT_VM(0);
+        ring_barrier();
+    };
+    const auto kfrag = [&](int u) {
+        const u32x4 *st = &ring[u % (STAGES * UPS)][lane];
+        return [st](int k, int ks) { return st[(2 * ks + k) * 64]; };
+    };
+    const auto vfrag = [&](int u) {
+        const u32x4 *st = &ring[u % (STAGES * UPS)][MT * 64 + lane];
+        return [st](int mt) { return st[mt * 64]; };
+    };
+    for (int s = 0; s < STAGES - 2 && s < ns; s++) issue(s);
+    typename W::Scores sc;
+    float mx[NQT];
+    arrive(0);
+    if (STAGES - 2 < ns) issue(STAGES - 2);
+    q.scores(sc, kfrag(0));
+    q.mend(sc, kfrag(0));
+    if (nc == 0) q.mask(sc, w.u0 * kTreeKeys);
+    q.largest(sc, mx);
+    // Before the scores of unit u + 1: its stage; then every wave is past the scores
+    // and values of the stage two before, whose place the next request takes.
+    auto ahead = [&](int u) {
+        if ((u + 1) % UPS) return;
+        const int s = (u + 1) / UPS;
+        arrive(s);
+        if (s + STAGES - 2 < ns) issue(s + STAGES - 2);
+    };
+    int u = 0;
+    for (; u + UPS < nc; u += UPS) {
+#pragma unroll
+        for (int i = 0; i < UPS; i++) {
+            q.grow(mx, a.qscale);
+            ahead(u + i);
+            typename W::Scores next;
+            typename W::Weights pw;
+            q.scores(next, kfrag(u + i + 1));
+            q.weights(sc, pw, a.qscale);
+            q.mend(next, kfrag(u + i + 1));
+            q.template values<false>(pw, 0, vfrag(u + i));
+            q.largest(next, mx);
+#pragma unroll
+            for (int nt = 0; nt < NQT; nt++) sc[nt][0] = next[nt][0], sc[nt][1] = next[nt][1];
+        }
+    }
+    for (; u < nu; u++) {
+        q.grow(mx, a.qscale);
+        typename W::Weights pw;
+        q.weights(sc, pw, a.qscale);
+        q.template values<true>(pw, (w.u0 + u) * kTreeKeys, vfrag(u));
+        if (u + 1 < nu) {
+            ahead(u);
+            q.scores(sc, kfrag(u + 1));
+            q.mend(sc, kfrag(u + 1));
+            q.mask(sc, (w.u0 + u + 1) * kTreeKeys);
+            q.largest(sc, mx);
+        }
+    }
+
+    const bool any_odd = __builtin_amdgcn_ballot_w64(q.odd) != 0;
+    const int64_t slot = tree_slot(w.R, a.KVH, w.tiles, w.split, w.kvh, w.tile);
+#pragma unroll
+    for (int nt = 0; nt < NQT; nt++) {
+        const int qt = (wave * NQT + nt) * 16 + q.col, qr = w.tile * QT + qt;
+        const float L = rows4_sum(q.l_part[nt]), inv = L > 0.f ? 1.f / L : 0.f;
+        if (qr >= w.QR) continue;
+        const int64_t base = tree_qbase(a, w.R, w.kvh, w.G, qr);
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            fl4 o = q.acc[nt][mt];
+            const int d0 = mt * 16 + q.grp * 4;
+            if (any_odd) q.add_odd(a, w, nt, d0, o);
+            if (w.R.nsplit > 1) {
+                *(fl4 *)(a.part_o + (slot * QT + qt) * D + d0) = o;
+            } else if (d0 < a.DQ) {
+                const float v[4] = {o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
+                tree_store4(a.out, base + d0, v, a.out_bf16);
+            }
+        }
+        if (w.R.nsplit > 1 && q.grp == 0) {
+            float *pm = a.part_ml + (slot * QT + qt) * 2;
+            pm[0] = q.m_run[nt];
             pm[1] = L;
         }
     }
@@ -493,10 +746,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(PlanArg plan, TreeArgs 
     const int Q4 = D >> 2, TQ = 256 / Q4, t = threadIdx.x;
     const int qr = blockIdx.z * TQ + t / Q4, d0 = (t - t / Q4 * Q4) * 4;
     if (t >= TQ * Q4 || qr >= QR) return;
-    const int tiles = (QR + QT - 1) / QT, streams = R.nsplit * a.KVH, tile = qr / QT, qt = qr - tile * QT;
-    const auto at = [&](int s) {
-        return ((int64_t)R.part + tree_place(s * a.KVH + kvh, tile, streams, tiles)) * QT + qt;
-    };
+    const int tiles = (QR + QT - 1) / QT, tile = qr / QT, qt = qr - tile * QT;
+    const auto at = [&](int s) { return tree_slot(R, a.KVH, tiles, s, kvh, tile) * QT + qt; };
     constexpr int kFew = 8;  // partials read in one round trip
     float M = -INFINITY, L = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -533,36 +784,54 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(PlanArg plan, TreeArgs 
 }
 
 int tree_tile_rows(int hd, int max_qr, bool fine) {
-    if (hd > 128 || max_qr <= 16) return 16;
-    return max_qr <= 32 || fine || hd > 64 ? 32 : 64;
+    if (max_qr <= 16) return 16;
+    if (hd < 64) return 32;  // the narrow kernel alone
+    if (max_qr <= 32 && hd < 256) return 32;
+    if (max_qr <= 64 || (hd == 256 && fine)) return 64;  // (registers)
+    return max_qr <= 128 || fine || hd == 256 ? 128 : 256;
 }
 
 hipError_t launch_tree_attend(hipStream_t s, const PlanArg &plan, const TreeArgs &a, int hd, int tile_rows,
                               bool fine, int n_wgs, bool merge, int max_qr, hipEvent_t e0, hipEvent_t e1) {
     if (n_wgs <= 0) return hipSuccess;
     void (*k)(PlanArg, TreeArgs) = nullptr;
-#define RLX_TREE_CASE(DD, NN)                                                              \
-    if (hd == DD && tile_rows == 16 * NN)                                                  \
-        k = fine ? tree_attend_kernel<DD, (NN < 4 ? NN : 2), true> : tree_attend_kernel<DD, NN, false>;
-    RLX_TREE_CASE(16, 1)
-    RLX_TREE_CASE(16, 2)
-    RLX_TREE_CASE(16, 4)
-    RLX_TREE_CASE(32, 1)
-    RLX_TREE_CASE(32, 2)
-    RLX_TREE_CASE(32, 4)
-    RLX_TREE_CASE(64, 1)
-    RLX_TREE_CASE(64, 2)
-    RLX_TREE_CASE(64, 4)
-    RLX_TREE_CASE(96, 1)
-    RLX_TREE_CASE(96, 2)
-    RLX_TREE_CASE(96, 4)
-    RLX_TREE_CASE(128, 1)
-    RLX_TREE_CASE(128, 2)
-    RLX_TREE_CASE(128, 4)
-    RLX_TREE_CASE(256, 1)
-#undef RLX_TREE_CASE
+#define RLX_TREE_NARROW(DD, NN) \
+    if (hd == DD && tile_rows == 16 * NN) k = fine ? tree_narrow_kernel<DD, NN, true> : tree_narrow_kernel<DD, NN, false>;
+#define RLX_TREE_WIDE(DD, NN, WW, FF) \
+    if (hd == DD && tile_rows == 16 * NN * WW && fine == FF) k = tree_wide_kernel<DD, NN, WW, FF>;
+    RLX_TREE_NARROW(16, 1)
+    RLX_TREE_NARROW(16, 2)
+    RLX_TREE_NARROW(32, 1)
+    RLX_TREE_NARROW(32, 2)
+    RLX_TREE_NARROW(64, 1)
+    RLX_TREE_NARROW(64, 2)
+    RLX_TREE_NARROW(96, 1)
+    RLX_TREE_NARROW(96, 2)
+    RLX_TREE_NARROW(128, 1)
+    RLX_TREE_NARROW(128, 2)
+    RLX_TREE_NARROW(256, 1)
+    RLX_TREE_WIDE(64, 1, 4, false)
+    RLX_TREE_WIDE(64, 1, 4, true)
+    RLX_TREE_WIDE(64, 1, 8, false)
+    RLX_TREE_WIDE(64, 1, 8, true)
+    RLX_TREE_WIDE(64, 2, 8, false)
+    RLX_TREE_WIDE(96, 1, 4, false)
+    RLX_TREE_WIDE(96, 1, 4, true)
+    RLX_TREE_WIDE(96, 1, 8, false)
+    RLX_TREE_WIDE(96, 1, 8, true)
+    RLX_TREE_WIDE(96, 2, 8, false)
+    RLX_TREE_WIDE(128, 1, 4, false)
+    RLX_TREE_WIDE(128, 1, 4, true)
+    RLX_TREE_WIDE(128, 1, 8, false)
+    RLX_TREE_WIDE(128, 1, 8, true)
+    RLX_TREE_WIDE(128, 2, 8, false)
+    RLX_TREE_WIDE(256, 1, 4, false)
+    RLX_TREE_WIDE(256, 1, 4, true)
+    RLX_TREE_WIDE(256, 1, 8, false)
+#undef RLX_TREE_NARROW
+#undef RLX_TREE_WIDE
     if (!k) return hipErrorInvalidValue;
-    hipError_t e = launch_timed(k, dim3(n_wgs), dim3(256), s, e0, e1, plan, a);
+    hipError_t e = launch_timed(k, dim3(n_wgs), dim3(tile_rows <= 64 ? 256 : 512), s, e0, e1, plan, a);
     if (e != hipSuccess || !merge) return e;
     const int TQ = 256 / (hd / 4);
     tree_merge_kernel<<<dim3(a.n_rows, a.KVH, (max_qr + TQ - 1) / TQ), 256, 0, s>>>(plan, a, hd, tile_rows);
