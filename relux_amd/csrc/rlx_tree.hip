@@ -56,7 +56,8 @@ __device__ __forceinline__ int64_t tree_qbase(const TreeArgs &a, const TreeRow &
 // Ancestor sets of a tree's nodes, bit k of word w of node j: node 32 w + k is j
 // or an ancestor.  Each round joins a node's set with that of the node it
 // points to and doubles how far it points (8 rounds for a chain of 256).  A
-// parent outside [0, j) ends the chain.
+// parent outside [0, j) ends the chain.  Words past the tree's are zero up to one
+// more than its last.
 __device__ __forceinline__ void tree_ancestors(const int32_t *parents, int n, uint32_t (*anc)[kTreeMaxNodes],
                                                int16_t *up) {
     const int j = threadIdx.x, words = (n + 31) >> 5;
@@ -64,7 +65,7 @@ __device__ __forceinline__ void tree_ancestors(const int32_t *parents, int n, ui
     if (j < n) {
         const int p = parents[j];
         u = p >= 0 && p < j ? p : -1;
-        for (int w = 0; w < words; w++) anc[w][j] = w == (j >> 5) ? 1u << (j & 31) : 0u;
+        for (int w = 0; w <= words; w++) anc[w][j] = w == (j >> 5) ? 1u << (j & 31) : 0u;
         up[j] = (int16_t)u;
     }
     while (__syncthreads_or(u >= 0)) {
@@ -187,8 +188,7 @@ __device__ __forceinline__ void tree_parts(float (&v)[8], u32x4 (&o)[PARTS]) {
 //
 // A masked weight is a selected zero; a value that is not finite in a masked
 // place must not reach other rows through 0 x inf, so such values of the tree's
-// keys stay out of the product and are added at the end to the rows that attend
-// them (an infinity or NaN whatever its weight).
+// keys stay out of the product and replace the sums of the rows that attend them.
 template <int D, int NQT, bool FINE, bool ACC>
 struct TreeWave {
     static constexpr int KS = D < 32 ? 1 : D / 32, MT = D / 16, PARTS = FINE ? 3 : 1;
@@ -249,12 +249,6 @@ struct TreeWave {
                 for (int p = 0; p < PARTS; p++) asm volatile("" ::"v"(qb[nt][ks][p]));
     }
 
-    __device__ __forceinline__ bool allowed(int t, int nt) const {
-        if (t < ctx) return true;
-        const int k = t - ctx;
-        return t < len && ((anc[k >> 5][node[nt]] >> (k & 31)) & 1u);
-    }
-
     typedef fl4 Scores[NQT][2];
     typedef u32x4 Weights[NQT][PARTS];
 
@@ -308,13 +302,25 @@ struct TreeWave {
             }
         }
     }
+    // The keys tl .. tl + 7 that row tile nt's row attends, as bits (none past the
+    // last token: it has no node there).
+    __device__ __forceinline__ uint32_t seen8(int tl, int nt) const {
+        const int k = tl - ctx;
+        if (k <= -8) return 0xFFu;
+        if (k < 0) return (anc[0][node[nt]] << -k) | ((1u << -k) - 1u);
+        const int w = min(k >> 5, kTreeMaxNodes / 32 - 1);
+        const uint64_t bits = (uint64_t)anc[w + 1][node[nt]] << 32 | anc[w][node[nt]];
+        return tl < len ? (uint32_t)(bits >> (k & 31)) : 0u;
+    }
     // Masks a unit from key t0 that holds keys of the tree, or past the last token.
     __device__ __forceinline__ void mask(Scores &s, int t0) const {
 #pragma unroll
-        for (int nt = 0; nt < NQT; nt++)
+        for (int nt = 0; nt < NQT; nt++) {
+            const uint32_t m = seen8(t0 + grp * 8, nt);
 #pragma unroll
             for (int i = 0; i < 8; i++)
-                if (!allowed(t0 + grp * 8 + i, nt)) s[nt][i >> 2][i & 3] = -INFINITY;
+                if (!(m & (1u << i))) s[nt][i >> 2][i & 3] = -INFINITY;
+        }
     }
     // A lane's largest scores.
     __device__ __forceinline__ void largest(const Scores &s, float (&mx)[NQT]) const {
@@ -372,46 +378,81 @@ struct TreeWave {
                 for (int i = 0; i < 4; i++) l_part[nt] = add_bf16x2(pw[nt][0][i], l_part[nt]);
         }
     }
-    // The values' product; vf(mt): their fragments.  TREE: as mask().
+    // The values' product; vf(mt): their fragments.  TREE: as mask(); values past the
+    // last token are zeroed, and those of the tree that are not finite taken out.
     template <bool TREE, class VF>
     __device__ __forceinline__ void values(const Weights &pw, int t0, VF vf) {
-        const int tl = t0 + grp * 8;
+        u32x4 v[MT];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            u32x4 v = vf(mt);
-            if constexpr (TREE) {
+        for (int mt = 0; mt < MT; mt++) v[mt] = vf(mt);
+        if constexpr (TREE) {
+            const int tl = t0 + grp * 8;
+            u32x4 live, tree;  // halves before the last token; of the tree
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const uint32_t keep = (i & 1) ? 0x0000FFFFu : 0xFFFF0000u, ex = 0x7F807F80u & ~keep;
-                    const bool inf = tl + i >= ctx && (v[i >> 1] & ex) == ex;
-                    odd |= inf && tl + i < len;
-                    if (tl + i >= len || inf) v[i >> 1] &= keep;
-                }
+            for (int i = 0; i < 4; i++) {
+                live[i] = (tl + 2 * i < len ? 0xFFFFu : 0u) | (tl + 2 * i + 1 < len ? 0xFFFF0000u : 0u);
+                tree[i] = (tl + 2 * i >= ctx ? 0x8000u : 0u) | (tl + 2 * i + 1 >= ctx ? 0x80000000u : 0u);
             }
+            uint32_t bad = 0;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    v[mt][i] &= live[i];
+                    bad |= ((v[mt][i] & 0x7F807F80u) + 0x00800080u) & tree[i];  // an exponent of ones carries
+                }
+            if (__builtin_amdgcn_ballot_w64(bad != 0)) {
+                odd = true;
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t x = ((v[mt][i] & 0x7F807F80u) + 0x00800080u) & tree[i];
+                        v[mt][i] &= ~((x >> 15) * 0xFFFFu);
+                    }
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
 #pragma unroll
             for (int p = PARTS - 1; p >= 0; p--)
 #pragma unroll
                 for (int nt = 0; nt < NQT; nt++)
                     acc[nt][mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, pw[nt][p]), acc[nt][mt], 0, 0, 0);
-        }
-    }
-
-    // The tree's values that are not finite, for dims d0 .. d0 + 3 of row tile nt.
-    __device__ __forceinline__ void add_odd(const TreeArgs &a, const TreeItem &w, int nt, int d0, fl4 &o) const {
-#pragma unroll 1
-        for (int t = max(w.u0 * kTreeKeys, ctx); t < min(w.u1 * kTreeKeys, len); t++) {
-            if (!allowed(t, nt)) continue;
-            const int e = t / a.P;
-            const uint16_t *vp = a.vpool + ((int64_t)a.table[w.R.tab + e] * a.KVH + w.kvh) * a.P * D + (t - e * a.P);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint16_t x = vp[(d0 + i) * a.P];
-                if ((x & 0x7F80) == 0x7F80) o[i] += bf16_f32(x);
-            }
-        }
+                        __builtin_bit_cast(bf16x8, v[mt]), __builtin_bit_cast(bf16x8, pw[nt][p]), acc[nt][mt], 0, 0, 0);
     }
 };
+
+// The tree's values that are not finite, taken out of the product: where the row qt
+// of the tile attends one in dims d0 .. d0 + 3 it is the sum, whatever the weights.
+// Run by the lane that stored these dims, after it.
+__device__ __forceinline__ void tree_odd(const TreeArgs &a, const TreeItem &w, const uint32_t (*anc)[kTreeMaxNodes],
+                                         int64_t slot, int D, int QT, int qt, int d0) {
+    const int qr = w.tile * QT + qt;
+    if (qr >= w.QR || (w.R.nsplit == 1 && d0 >= a.DQ)) return;
+    const int node = w.nodes - w.nq + qr / w.G;
+#pragma unroll 1
+    for (int i = 0; i < 4; i++) {
+        float x = 0.f;
+#pragma unroll 1
+        for (int t = max(w.u0 * kTreeKeys, w.ctx); t < min(w.u1 * kTreeKeys, w.R.len); t++) {
+            const int k = t - w.ctx, e = t / a.P;
+            if (!((anc[k >> 5][node] >> (k & 31)) & 1u)) continue;
+            const uint16_t v = a.vpool[(((int64_t)a.table[w.R.tab + e] * a.KVH + w.kvh) * D + d0 + i) * a.P + (t - e * a.P)];
+            if ((v & 0x7F80) == 0x7F80) x += bf16_f32(v);
+        }
+        if (x == 0.f) continue;
+        if (w.R.nsplit > 1) {
+            a.part_o[(slot * QT + qt) * D + d0 + i] = x;
+        } else {
+            const int64_t o = tree_qbase(a, w.R, w.kvh, w.G, qr) + d0 + i;
+            if (a.out_bf16)
+                ((uint16_t *)a.out)[o] = bf16_rne(x);
+            else
+                ((float *)a.out)[o] = x;
+        }
+    }
+}
 
 // Byte offsets into the K and V pools of a lane's block (lane & 1) of unit j +
 // lane / 2, of `nu` units `step` apart from unit `first`.  A block past the last
@@ -466,7 +507,7 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
     using W = TreeWave<D, NQT, FINE, true>;
     constexpr int KS = W::KS, MT = W::MT, QT = 16 * NQT;
     constexpr int MC = MT < 8 ? MT : 8;  // m-tiles merged at a time
-    __shared__ uint32_t anc[kTreeMaxNodes / 32][kTreeMaxNodes];
+    __shared__ uint32_t anc[kTreeMaxNodes / 32 + 1][kTreeMaxNodes];
     __shared__ int16_t up[kTreeMaxNodes];
     __shared__ float sm[4][QT], sl[4][QT];
     __shared__ fl4 so[4][MC][64];
@@ -572,10 +613,10 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
 #pragma unroll
             for (int mt = 0; mt < MC; mt++) so[wave][mt][lane] = q.acc[nt][m0 + mt] * f;
             __syncthreads();
+#pragma unroll 1
             for (int mt = wave; mt < MC; mt += 4) {
-                fl4 o = (so[0][mt][lane] + so[1][mt][lane]) + (so[2][mt][lane] + so[3][mt][lane]);
+                const fl4 o = (so[0][mt][lane] + so[1][mt][lane]) + (so[2][mt][lane] + so[3][mt][lane]);
                 const int d0 = (m0 + mt) * 16 + q.grp * 4;
-                if (any_odd) q.add_odd(a, w, nt, d0, o);
                 if (w.R.nsplit > 1) {
                     *(fl4 *)(a.part_o + (slot * QT + qt) * D + d0) = o;
                 } else if (qr < w.QR && d0 < a.DQ) {
@@ -589,6 +630,13 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
             pm[0] = M;
             pm[1] = L;
         }
+    }
+    if (any_odd) {
+#pragma unroll 1
+        for (int nt = 0; nt < NQT; nt++)
+#pragma unroll 1
+            for (int mt = wave; mt < MT; mt += 4)
+                tree_odd(a, w, anc, slot, D, QT, nt * 16 + q.col, mt * 16 + q.grp * 4);
     }
 }
 
@@ -608,7 +656,7 @@ __global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void t
     constexpr int STAGES = 4;                               // of 16 KB a unit (D 128) or 32
     constexpr int SLABS = UPS * 2 * MT, LOADS = (SLABS + WAVES - 1) / WAVES;  // fragments of a stage; a wave's of them
     static_assert(SLABS % WAVES == 0 && MT % LOADS == 0, "a wave loads K or V");
-    __shared__ uint32_t anc[kTreeMaxNodes / 32][kTreeMaxNodes];
+    __shared__ uint32_t anc[kTreeMaxNodes / 32 + 1][kTreeMaxNodes];
     __shared__ int16_t up[kTreeMaxNodes];
     __shared__ u32x4 ring[STAGES * UPS][UNIT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -719,9 +767,8 @@ __global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void t
         const int64_t base = tree_qbase(a, w.R, w.kvh, w.G, qr);
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            fl4 o = q.acc[nt][mt];
+            const fl4 o = q.acc[nt][mt];
             const int d0 = mt * 16 + q.grp * 4;
-            if (any_odd) q.add_odd(a, w, nt, d0, o);
             if (w.R.nsplit > 1) {
                 *(fl4 *)(a.part_o + (slot * QT + qt) * D + d0) = o;
             } else if (d0 < a.DQ) {
@@ -734,6 +781,11 @@ __global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void t
             pm[0] = q.m_run[nt];
             pm[1] = L;
         }
+    }
+    if (any_odd) {
+#pragma unroll 1
+        for (int i = 0; i < NQT * MT; i++)
+            tree_odd(a, w, anc, slot, D, QT, (wave * NQT + i / MT) * 16 + q.col, i % MT * 16 + q.grp * 4);
     }
 }
 
@@ -787,8 +839,8 @@ int tree_tile_rows(int hd, int max_qr, bool fine) {
     if (max_qr <= 16) return 16;
     if (hd < 64) return 32;  // the narrow kernel alone
     if (max_qr <= 32 && hd < 256) return 32;
-    if (max_qr <= 64 || (hd == 256 && fine)) return 64;  // (registers)
-    return max_qr <= 128 || fine || hd == 256 ? 128 : 256;
+    if (max_qr <= 64 || hd == 256) return 64;  // (registers)
+    return max_qr <= 128 || fine ? 128 : 256;
 }
 
 hipError_t launch_tree_attend(hipStream_t s, const PlanArg &plan, const TreeArgs &a, int hd, int tile_rows,
@@ -827,7 +879,6 @@ hipError_t launch_tree_attend(hipStream_t s, const PlanArg &plan, const TreeArgs
     RLX_TREE_WIDE(128, 2, 8, false)
     RLX_TREE_WIDE(256, 1, 4, false)
     RLX_TREE_WIDE(256, 1, 4, true)
-    RLX_TREE_WIDE(256, 1, 8, false)
 #undef RLX_TREE_NARROW
 #undef RLX_TREE_WIDE
     if (!k) return hipErrorInvalidValue;
