@@ -58,13 +58,11 @@ __device__ __forceinline__ int64_t tree_qbase(const TreeArgs &a, const TreeRow &
 // points to and doubles how far it points (8 rounds for a chain of 256).  A
 // parent outside [0, j) ends the chain.  Words past the tree's are zero up to one
 // more than its last.
-__device__ __forceinline__ void tree_ancestors(const int32_t *parents, int n, uint32_t (*anc)[kTreeMaxNodes],
-                                               int16_t *up) {
+__device__ __forceinline__ void tree_ancestors(int parent, int n, uint32_t (*anc)[kTreeMaxNodes], int16_t *up) {
     const int j = threadIdx.x, words = (n + 31) >> 5;
     int u = -1;
     if (j < n) {
-        const int p = parents[j];
-        u = p >= 0 && p < j ? p : -1;
+        u = parent >= 0 && parent < j ? parent : -1;
         for (int w = 0; w <= words; w++) anc[w][j] = w == (j >> 5) ? 1u << (j & 31) : 0u;
         up[j] = (int16_t)u;
     }
@@ -460,16 +458,25 @@ __device__ __forceinline__ void tree_odd(const TreeArgs &a, const TreeItem &w, c
 template <int D>
 struct TreePages {
     int64_t k, v;
-    __device__ __forceinline__ void fetch(const TreeArgs &a, const TreeItem &w, int first, int step, int nu, int j) {
+    int page, slot;
+    __device__ __forceinline__ void request(const TreeArgs &a, const TreeItem &w, int first, int step, int nu, int j) {
         const int lane = threadIdx.x & 63;
         int t = (first + step * min(j + (lane >> 1), nu - 1)) * kTreeKeys + 16 * (lane & 1);
         t = min(t, (w.R.len - 1) & ~15);
-        const int e = a.pshift >= 0 ? t >> a.pshift : t / a.P, slot = t - e * a.P;
-        const int64_t base = ((int64_t)a.table[w.R.tab + e] * a.KVH + w.kvh) * a.P * D;
+        const int e = a.pshift >= 0 ? t >> a.pshift : t / a.P;
+        slot = t - e * a.P;
+        page = a.table[w.R.tab + e];
+    }
+    __device__ __forceinline__ void take(const TreeArgs &a, const TreeItem &w) {
+        const int64_t base = ((int64_t)page * a.KVH + w.kvh) * a.P * D;
         k = (base + (int64_t)slot * D) * 2;
         v = (base + slot) * 2;
         // wait here, so that no wait for these sits on the common path
         asm volatile("" ::"v"(k), "v"(v));
+    }
+    __device__ __forceinline__ void fetch(const TreeArgs &a, const TreeItem &w, int first, int step, int nu, int j) {
+        request(a, w, first, step, nu, j);
+        take(a, w);
     }
     // A lane's offset in unit j of the fetched ones: that of its block.
     static __device__ __forceinline__ int64_t pick(int64_t off, int j, bool second) {
@@ -514,15 +521,16 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TreeItem w;
     if (!tree_item<QT>(a, w)) return;
-    if (w.u1 * kTreeKeys > w.ctx) tree_ancestors(a.parents + w.R.node0, w.nodes, anc, up);
+    const int parent = threadIdx.x < w.nodes ? a.parents[w.R.node0 + threadIdx.x] : -1;
 
     const int first = w.u0 + wave, nu = first < w.u1 ? (w.u1 - first + 3) / 4 : 0;
     const int nc = max(0, min(nu, (w.ctx / kTreeKeys - first + 3) / 4));  // units before the tree's
     TreePages<D> pages;
-    if (nu > 0) pages.fetch(a, w, first, 4, nu, 0);
+    if (nu > 0) pages.request(a, w, first, 4, nu, 0);
     const TreeLane<D> at(a);
     W q;
     q.init(a, w, w.tile * QT, anc);
+    if (nu > 0) pages.take(a, w);
 
     auto load = [&](int j, u32x4(&kr)[2][KS], u32x4(&vr)[MT]) {
         j = min(j, nu - 1);
@@ -558,8 +566,10 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
     // dim 256 has registers for one.
     u32x4 ka[2][KS], kb[2][KS], va[MT], vb[MT];
     int j = 0;
-    if constexpr (D <= 128) {
+    if constexpr (D <= 128)
         if (nu > 0) load(0, ka, va);
+    if (w.u1 * kTreeKeys > w.ctx) tree_ancestors(parent, w.nodes, anc, up);
+    if constexpr (D <= 128) {
         q.ready();
         for (; j + 1 < nc; j += 2) {
             load(j + 1, kb, vb);
@@ -662,23 +672,25 @@ __global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void t
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TreeItem w;
     if (!tree_item<QT>(a, w)) return;
-    if (w.u1 * kTreeKeys > w.ctx) tree_ancestors(a.parents + w.R.node0, w.nodes, anc, up);
+    const int parent = threadIdx.x < w.nodes ? a.parents[w.R.node0 + threadIdx.x] : -1;
 
     const int nu = w.u1 - w.u0;
     const int nc = max(0, min(nu, w.ctx / kTreeKeys - w.u0));  // units before the tree's
     const bool shared = w.QR > QT;  // other tiles read the same keys
     const uint32_t ring_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4 *)&ring[0][0];
     TreePages<D> pages;
+    pages.request(a, w, w.u0, 1, nu, 0);
     const TreeLane<D> at(a);
     W q;
     q.init(a, w, w.tile * QT + wave * 16 * NQT, anc);
     q.ready();
+    pages.take(a, w);
     const int ns = (nu + UPS - 1) / UPS;
     // a wave's fragments are of one unit, and of K or V alone
     const int i0 = wave * LOADS % (2 * MT), uu = wave * LOADS / (2 * MT);
     const bool is_v = i0 >= MT;
     auto issue = [&](int s) {
-        if ((s * UPS & 31) == 0) pages.fetch(a, w, w.u0, 1, nu, s * UPS);
+        if ((s * UPS & 31) == 0 && s) pages.fetch(a, w, w.u0, 1, nu, s * UPS);
         const uint32_t dst = ring_lds + (uint32_t)(s % STAGES * UPS * UNIT + wave * LOADS * 64) * 16;
         const char *src = is_v ? at.v + pages.pick(pages.v, s * UPS + uu, at.v2) + (i0 - MT) * a.P * 32
                                : at.k + pages.pick(pages.k, s * UPS + uu, at.k2);
@@ -710,6 +722,7 @@ __global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void t
         return [st](int mt) { return st[mt * 64]; };
     };
     for (int s = 0; s < STAGES - 2 && s < ns; s++) issue(s);
+    if (w.u1 * kTreeKeys > w.ctx) tree_ancestors(parent, w.nodes, anc, up);
     typename W::Scores sc;
     float mx[NQT];
     arrive(0);
