@@ -3269,8 +3269,6 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
     const int G = num_heads / c->kvh;
     const bool fine = q_dtype == RLX_F32 || out_dtype == RLX_F32;
     int max_qr = 0;
-    for (int i = 0; i < n_seqs; i++) max_qr = std::max(max_qr, G * (n_q ? n_q[i] : n_nodes[i]));
-    const int qt = tree_tile_rows(c->hd, max_qr, fine);
     std::vector<TreeRow> rows(n_seqs);
     std::vector<TreeLoad> load(n_seqs);
     int qrow = 0, node0 = 0;
@@ -3283,11 +3281,15 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
         r.nodes = n_nodes[i] | nq << 16;
         r.qrow = qrow;
         r.node0 = node0;
-        load[i] = TreeLoad{s.len, (nq * G + qt - 1) / qt, nq * G};
+        load[i] = TreeLoad{s.len, nq * G};
+        max_qr = std::max(max_qr, nq * G);
         qrow += nq;
         node0 += n_nodes[i];
     }
-    const std::vector<int> cuts = tree_cuts(load, c->kvh, c->cus, qt, c->hd, fine);
+    const TreePlan tp = tree_plan(load, c->kvh, c->cus, c->hd, fine);
+    const std::vector<int> &cuts = tp.cuts;
+    const int qt = tp.tile;
+    const auto tiles = [&](int i) { return (load[i].rows + qt - 1) / qt; };
     int64_t wgs = 0, parts = 0, n_cuts = 0;
     int max_tiles = 1;
     bool merge = false;
@@ -3296,7 +3298,7 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
     for (int i = 0; i < n_seqs; i++) {
         order[i] = i;
         n_cuts += cuts[i];
-        max_tiles = std::max(max_tiles, load[i].tiles);
+        max_tiles = std::max(max_tiles, tiles(i));
     }
     std::stable_sort(order.begin(), order.end(), [&](int x, int y) {
         return (int64_t)load[x].len * cuts[y] > (int64_t)load[y].len * cuts[x];
@@ -3306,7 +3308,7 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
     int at = 0;
     for (int k = 0; k < n_seqs; k++) {
         const int i = order[k];
-        const int64_t n = (int64_t)load[i].tiles * c->kvh * cuts[i];
+        const int64_t n = (int64_t)tiles(i) * c->kvh * cuts[i];
         by_cut[k] = rows[i];
         by_cut[k].nsplit = cuts[i];
         by_cut[k].at0 = spread ? at : (int32_t)wgs;
@@ -3333,7 +3335,7 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
         std::vector<int32_t> work;
         for (int k = 0; k < n_seqs; k++) {
             const int i = order[k];
-            work.insert(work.end(), spread ? cuts[i] : load[i].tiles * c->kvh * cuts[i], k);
+            work.insert(work.end(), spread ? cuts[i] : tiles(i) * c->kvh * cuts[i], k);
         }
         Blob b;
         const size_t o_r = b.add(rows), o_w = b.add(work);

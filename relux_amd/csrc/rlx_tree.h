@@ -36,8 +36,6 @@ struct TreeArgs {
     float qscale;                 // scale * log2(e)
 };
 
-// Query rows of a tile.
-int tree_tile_rows(int hd, int max_qr, bool fine);
 // fine: queries and weights in parts of bf16, for f32 queries or outputs.
 hipError_t launch_tree_attend(hipStream_t s, const PlanArg &plan, const TreeArgs &a, int hd, int tile_rows,
                               bool fine, int n_wgs, bool merge, int max_qr, hipEvent_t e0, hipEvent_t e1);

@@ -509,7 +509,8 @@ struct TreeLane {
 // Few query rows: 4 waves, each holding all 16 NQT rows of the tile and taking
 // every fourth unit, straight from HBM into registers in the operands' order -- no
 // LDS and no barrier in the loop.  HBM-bound.
-template <int D, int NQT, bool FINE>
+// SHARED: other tiles read the same keys, which stay in L2 (else non-temporal loads).
+template <int D, int NQT, bool FINE, bool SHARED>
 __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeArgs a) {
     using W = TreeWave<D, NQT, FINE, true>;
     constexpr int KS = W::KS, MT = W::MT, QT = 16 * NQT;
@@ -532,6 +533,12 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
     q.init(a, w, w.tile * QT, anc);
     if (nu > 0) pages.take(a, w);
 
+    const auto get = [](const char *p) {
+        if constexpr (SHARED)
+            return *(const u32x4 *)p;
+        else
+            return __builtin_nontemporal_load((const u32x4 *)p);
+    };
     auto load = [&](int j, u32x4(&kr)[2][KS], u32x4(&vr)[MT]) {
         j = min(j, nu - 1);
         if ((j & 31) == 0 && j) pages.fetch(a, w, first, 4, nu, j);
@@ -540,9 +547,9 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
         for (int ks = 0; ks < KS; ks++)
 #pragma unroll
             for (int k = 0; k < 2; k++)
-                kr[k][ks] = __builtin_nontemporal_load((const u32x4 *)(kp + ks * at.kStep + k * at.kKeys4));
+                kr[k][ks] = get(kp + ks * at.kStep + k * at.kKeys4);
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) vr[mt] = __builtin_nontemporal_load((const u32x4 *)(vp + mt * a.P * 32));
+        for (int mt = 0; mt < MT; mt++) vr[mt] = get(vp + mt * a.P * 32);
     };
     auto consume = [&](auto tree, int j, u32x4(&kr)[2][KS], u32x4(&vr)[MT]) {
         constexpr bool TREE = decltype(tree)::value;
@@ -848,20 +855,15 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(PlanArg plan, TreeArgs 
     tree_store4(a.out, tree_qbase(a, R, kvh, G, qr) + d0, v, a.out_bf16);
 }
 
-int tree_tile_rows(int hd, int max_qr, bool fine) {
-    if (max_qr <= 16) return 16;
-    if (hd < 64) return 32;  // the narrow kernel alone
-    if (max_qr <= 32 && hd < 256) return 32;
-    if (max_qr <= 64 || hd == 256) return 64;  // (registers)
-    return max_qr <= 128 || fine ? 128 : 256;
-}
-
 hipError_t launch_tree_attend(hipStream_t s, const PlanArg &plan, const TreeArgs &a, int hd, int tile_rows,
                               bool fine, int n_wgs, bool merge, int max_qr, hipEvent_t e0, hipEvent_t e1) {
     if (n_wgs <= 0) return hipSuccess;
     void (*k)(PlanArg, TreeArgs) = nullptr;
-#define RLX_TREE_NARROW(DD, NN) \
-    if (hd == DD && tile_rows == 16 * NN) k = fine ? tree_narrow_kernel<DD, NN, true> : tree_narrow_kernel<DD, NN, false>;
+    const bool shared = max_qr > tile_rows;
+#define RLX_TREE_NARROW(DD, NN)                                                                                   \
+    if (hd == DD && tile_rows == 16 * NN)                                                                         \
+        k = fine ? (shared ? tree_narrow_kernel<DD, NN, true, true> : tree_narrow_kernel<DD, NN, true, false>)    \
+                 : (shared ? tree_narrow_kernel<DD, NN, false, true> : tree_narrow_kernel<DD, NN, false, false>);
 #define RLX_TREE_WIDE(DD, NN, WW, FF) \
     if (hd == DD && tile_rows == 16 * NN * WW && fine == FF) k = tree_wide_kernel<DD, NN, WW, FF>;
     RLX_TREE_NARROW(16, 1)
