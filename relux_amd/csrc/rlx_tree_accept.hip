@@ -20,8 +20,9 @@
 // Without draft logits a draft is a choice without a distribution (q_i = the
 // child's token): accepted when u A_i < p(x), else its probability is removed.
 //
-// Weights are e = exp2((l - max) log2(e) / T) in f32, sums over the vocabulary in
-// f64: a draw's place among V tokens moves by V times a sum's rounding.
+// Weights are exp2((l - m) log2(e) / T) in f32, m near the row's maximum, sums over
+// the vocabulary in f64: a draw's place among V tokens moves by V times a sum's
+// rounding.
 #include "rlx_tree.h"
 
 namespace rlx {
@@ -33,9 +34,9 @@ namespace {
 
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// Entries i .. i + 3 of a row, -inf past the end.
-__device__ __forceinline__ float4 acc_load4(const float *row, int i, int end) {
-    if (i + 4 <= end) {
+// Entries i .. i + 3 of a row's [0, end): `full`, all inside; else -inf past the end.
+__device__ __forceinline__ float4 acc_load4(const float *row, int i, int end, bool full) {
+    if (full) {
         const f4u v = *(const f4u *)(row + i);
         return make_float4(v[0], v[1], v[2], v[3]);
     }
@@ -43,38 +44,58 @@ __device__ __forceinline__ float4 acc_load4(const float *row, int i, int end) {
     if (i < end) v.x = row[i];
     if (i + 1 < end) v.y = row[i + 1];
     if (i + 2 < end) v.z = row[i + 2];
+    if (i + 3 < end) v.w = row[i + 3];
     return v;
 }
 
-__device__ __forceinline__ float acc_e(float l, float m, float k) { return __builtin_amdgcn_exp2f((l - m) * k); }
+// Weight of a logit: exp2(l k - m k), mk = m k rounded once for the whole row.
+__device__ __forceinline__ float acc_e(float l, float k, float mk) { return __builtin_amdgcn_exp2f(fmaf(l, k, -mk)); }
 
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
 
-// A thread's running maximum and sum of exp2((l - max) k).
+constexpr int kAccBatch = 4;  // float4 of a row a lane has in flight
+
+// A wave's sum of exp2(l k - mk), mk of the wave's first batch's maximum unless a
+// later entry exceeds it by 2^60.
 struct Online {
-    float m = -INFINITY;
-    double s = 0.0;
-    __device__ __forceinline__ void add(const float4 &v, float k) {
-        const float x = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-        if (x > m) {
-            s *= (double)acc_e(m, x, k);
-            m = x;
+    float mk = 0.f;
+    double s = 0.0;  // this lane's
+    __device__ __forceinline__ void add(const float4 (&v)[kAccBatch], float k, bool first) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kAccBatch; i++) x = fmaxf(x, fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w)));
+        if (first || __builtin_amdgcn_ballot_w64(x * k > mk + 60.f)) {
+            const float m = wave_max(x) * k, to = m == -INFINITY ? 0.f : m;
+            if (!first) s *= (double)__builtin_amdgcn_exp2f(mk - to);
+            mk = to;
         }
-        if (m > -INFINITY) s += (double)((acc_e(v.x, m, k) + acc_e(v.y, m, k)) + (acc_e(v.z, m, k) + acc_e(v.w, m, k)));
+        float sum[kAccBatch];
+#pragma unroll
+        for (int i = 0; i < kAccBatch; i++)
+            sum[i] = (acc_e(v[i].x, k, mk) + acc_e(v[i].y, k, mk)) + (acc_e(v[i].z, k, mk) + acc_e(v[i].w, k, mk));
+        s += (double)((sum[0] + sum[1]) + (sum[2] + sum[3]));
     }
 };
 
 struct RowStat {
-    float m;
+    float mk;
     double z;
 };
 
 }  // namespace
 
+// One work-group a sequence: the walk reads the rows of the accepted path alone, each
+// once the node before it is decided.  Bound by that chain: of each pass the
+// exponentials of V / 4 entries a SIMD, behind a row's memory latency.
 template <bool Q>
 __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, TreeAcceptArgs a) {
     __shared__ int par[kTreeMaxNodes], tok[kTreeMaxNodes], gone[kTreeMaxNodes], way[kTreeMaxNodes];
@@ -103,33 +124,46 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
     int cur = 0, steps = 0, n_gone = 0;
     if (tid == 0) way[0] = 0;
     const float *t, *d;
-    RowStat T, D{0.f, 1.0};
+    RowStat T{0.f, 0.0}, D{0.f, 1.0};
     double C, S, A;  // A in units of the target's weights (p's mass = T.z)
     float ratio;     // C in those units: max(0, e_t - ratio e_q)
-    auto rest = [&](float et, float eq) { return Q && eq > 0.f ? fmaxf(0.f, fmaf(-ratio, eq, et)) : et; };
+    auto rest = [&](float et, float eq) __attribute__((always_inline)) {
+        return Q ? fmaxf(0.f, fmaf(-ratio, eq, et)) : et;
+    };
+    auto load = [&](const float *row, float4 (&v)[kAccBatch], int base, int end) __attribute__((always_inline)) {
+        const bool full = base + kAccBatch * 256 <= end;
+#pragma unroll
+        for (int i = 0; i < kAccBatch; i++) v[i] = acc_load4(row, base + i * 256 + lane * 4, end, full);
+    };
     // Sum of what remains of entries [lo, hi) by this wave's lanes, the rejected
     // tokens left out where they have no distribution.
     auto mass = [&](int lo, int hi) {
         double s = 0.0;
-        for (int base = lo; base < hi; base += 256) {
-            const int i = base + lane * 4;
-            const float4 x = acc_load4(t, i, hi);
-            float e[4] = {acc_e(x.x, T.m, k), acc_e(x.y, T.m, k), acc_e(x.z, T.m, k), acc_e(x.w, T.m, k)};
-            if constexpr (Q) {
-                const float4 y = acc_load4(d, i, hi);
-                e[0] = rest(e[0], acc_e(y.x, D.m, k));
-                e[1] = rest(e[1], acc_e(y.y, D.m, k));
-                e[2] = rest(e[2], acc_e(y.z, D.m, k));
-                e[3] = rest(e[3], acc_e(y.w, D.m, k));
-            } else {
-                for (int g = 0; g < n_gone; g++) {
-                    const int at = gone[g] - i;
+        for (int base = lo; base < hi; base += kAccBatch * 256) {
+            float4 x[kAccBatch], y[kAccBatch];
+            load(t, x, base, hi);
+            if (Q && ratio > 0.f) load(d, y, base, hi);
+            float sum[kAccBatch];
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        if (at == c) e[c] = 0.f;
+            for (int i = 0; i < kAccBatch; i++) {
+                float e[4] = {acc_e(x[i].x, k, T.mk), acc_e(x[i].y, k, T.mk), acc_e(x[i].z, k, T.mk), acc_e(x[i].w, k, T.mk)};
+                if (Q && ratio > 0.f) {
+                    e[0] = rest(e[0], acc_e(y[i].x, k, D.mk));
+                    e[1] = rest(e[1], acc_e(y[i].y, k, D.mk));
+                    e[2] = rest(e[2], acc_e(y[i].z, k, D.mk));
+                    e[3] = rest(e[3], acc_e(y[i].w, k, D.mk));
                 }
+                if (!Q) {
+                    for (int g = 0; g < n_gone; g++) {
+                        const int at = gone[g] - (base + i * 256 + lane * 4);
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+                            if (at == c) e[c] = 0.f;
+                    }
+                }
+                sum[i] = (e[0] + e[1]) + (e[2] + e[3]);
             }
-            s += (double)((e[0] + e[1]) + (e[2] + e[3]));
+            s += (double)((sum[0] + sum[1]) + (sum[2] + sum[3]));
         }
         return s;
     };
@@ -160,39 +194,39 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
             lt[tid] = t[tok[tid]];
             if (Q) lq[tid] = d[tok[tid]];
         }
-        // maximum and mass of both rows in one pass
+        // the rows' masses (the draft's only where there are children)
+        const bool parent = Q && (kids[0] | kids[1] | kids[2] | kids[3]);
         {
             Online ot, oq;
-            for (int base = v0; base < v1; base += 256) {
-                ot.add(acc_load4(t, base + lane * 4, v1), k);
-                if (Q) oq.add(acc_load4(d, base + lane * 4, v1), k);
+            for (int base = v0; base < v1; base += kAccBatch * 256) {
+                float4 x[kAccBatch], y[kAccBatch];
+                load(t, x, base, v1);
+                if (parent) load(d, y, base, v1);
+                ot.add(x, k, base == v0);
+                if (parent) oq.add(y, k, base == v0);
             }
             auto fold = [&](Online &o, int side) {
-                float m = o.m;
-#pragma unroll
-                for (int s = 32; s > 0; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
-                const double z = wave_sum(o.m == -INFINITY ? 0.0 : o.s * (double)acc_e(o.m, m, k));
+                const double z = wave_sum(o.s);
                 if (lane == 0) {
-                    red_m[side][wave] = m;
+                    red_m[side][wave] = v0 < v1 ? o.mk : -INFINITY;
                     red_s[side][wave] = z;
                 }
             };
             fold(ot, 0);
-            if (Q) fold(oq, 1);
+            if (parent) fold(oq, 1);
             __syncthreads();
             auto join = [&](int side) {
                 RowStat r{-INFINITY, 0.0};
 #pragma unroll
-                for (int w = 0; w < kAccWaves; w++) r.m = fmaxf(r.m, red_m[side][w]);
-                if (r.m == -INFINITY) r.m = 0.f;
+                for (int w = 0; w < kAccWaves; w++) r.mk = fmaxf(r.mk, red_m[side][w]);
 #pragma unroll
-                for (int w = 0; w < kAccWaves; w++) r.z += red_s[side][w] * (double)acc_e(red_m[side][w], r.m, k);
+                for (int w = 0; w < kAccWaves; w++) r.z += red_s[side][w] * (double)__builtin_amdgcn_exp2f(red_m[side][w] - r.mk);
                 return r;
             };
             T = join(0);
-            if (Q) D = join(1);
+            if (parent) D = join(1);
             turn ^= 1;
-            if (tid < kAccWaves) part[turn][tid] = red_s[0][tid] * (double)acc_e(red_m[0][tid], T.m, k);
+            if (tid < kAccWaves) part[turn][tid] = red_s[0][tid] * (double)__builtin_amdgcn_exp2f(red_m[0][tid] - T.mk);
             __syncthreads();
         }
         C = 0.0;
@@ -211,9 +245,9 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
                 bool skip = x < 0 || x >= V;  // no token: rejected without effect, as a rejected token again is
                 for (int g = 0; g < n_gone; g++) skip |= gone[g] == x;
                 if (skip) continue;
-                const float et = acc_e(lt[c], T.m, k);
+                const float et = acc_e(lt[c], k, T.mk);
                 if constexpr (Q) {
-                    const float eq = acc_e(lq[c], D.m, k);
+                    const float eq = acc_e(lq[c], k, D.mk);
                     const double qx = (double)eq / D.z, px = (double)rest(et, eq);
                     if (S > 0.0 ? (double)uni[c] * qx * A < px * S : px > 0.0) {
                         went = c;
@@ -222,7 +256,7 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
                     if (S > 0.0) {
                         C += A / T.z / S;
                         S -= qx;
-                        ratio = (float)(C * T.z / D.z);
+                        ratio = (float)fmin(C * T.z / D.z, 3e38);  // (finite: 0 where a draft weight is 0)
                         A = total();
                         if (!(A > 0.0)) {  // nothing is left by rounding alone
                             C = 0.0;
@@ -253,62 +287,76 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
     // ---- the next token: the first whose cumulated mass exceeds u A --------------
     if (!Q && n_gone) A = total();
     double want = (double)uni[0] * A;
-    // The part of `n` sums where `want` falls (else the last one that holds any),
-    // want becoming what is left of it there.
-    auto pick = [&](const double *s) {
-        double c = 0.0;
-        int last = 0;
-        double before = 0.0;
-#pragma unroll 1
-        for (int w = 0; w < kAccWaves; w++) {
-            const double x = s[w];
-            if (!(x > 0.0)) continue;
-            last = w;
-            before = c;
-            c += x;
-            if (c > want) break;
+    // Which of the waves' sums `want` falls in (else the last that holds any); want
+    // becomes what is left of it there.
+    auto pick = [&](const double *sums) {
+        const double s = lane < kAccWaves ? fmax(sums[lane], 0.0) : 0.0;
+        double c = s;
+#pragma unroll
+        for (int o = 1; o < kAccWaves; o <<= 1) {
+            const double up = __shfl_up(c, o);
+            if (lane >= o) c += up;
         }
-        want -= before;
-        return last;
+        const uint64_t any = __builtin_amdgcn_ballot_w64(s > 0.0), over = __builtin_amdgcn_ballot_w64(s > 0.0 && c > want);
+        const int w = over ? __builtin_ctzll(over) : any ? 63 - __builtin_clzll(any) : 0;
+        want -= __shfl(c - s, w);
+        return w;
     };
+    // the wave's span again by all the waves, then a part of it by one
     int lo = pick(part[turn]) * span;
     const int sub = span / kAccWaves, hi = min(V, lo + span);
+    const int s0 = min(hi, lo + wave * sub), s1 = min(hi, s0 + sub);
     {
-        const int s0 = min(hi, lo + wave * sub), s1 = min(hi, s0 + sub);
         const double s = wave_sum(mass(s0, s1));
         turn ^= 1;
         if (lane == 0) part[turn][wave] = s;
-        __syncthreads();
-        lo += pick(part[turn]) * sub;
     }
-    if (wave == 0) {
-        const int end = min(hi, lo + sub);
+    __syncthreads();
+    const int owner = pick(part[turn]);
+    if (wave == owner) {
         int found = -1, some = -1;
-        for (int base = lo; base < end && found < 0; base += 64) {
-            const int i = base + lane;
-            float e = 0.f;
-            if (i < end) {
-                e = acc_e(t[i], T.m, k);
-                if (Q) e = rest(e, acc_e(d[i], D.m, k));
-                for (int g = 0; !Q && g < n_gone; g++)
-                    if (gone[g] == i) e = 0.f;
+        for (int base = s0; base < s1 && found < 0; base += 256) {
+            const int at = base + lane * 4;
+            const bool full = base + 256 <= s1;
+            const float4 x = acc_load4(t, at, s1, full);
+            float e[4] = {acc_e(x.x, k, T.mk), acc_e(x.y, k, T.mk), acc_e(x.z, k, T.mk), acc_e(x.w, k, T.mk)};
+            if (Q && ratio > 0.f) {
+                const float4 y = acc_load4(d, at, s1, full);
+                e[0] = rest(e[0], acc_e(y.x, k, D.mk));
+                e[1] = rest(e[1], acc_e(y.y, k, D.mk));
+                e[2] = rest(e[2], acc_e(y.z, k, D.mk));
+                e[3] = rest(e[3], acc_e(y.w, k, D.mk));
             }
-            double c = (double)e;
+            for (int g = 0; !Q && g < n_gone; g++)
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+                    if (gone[g] == at + c) e[c] = 0.f;
+            const double s = (double)((e[0] + e[1]) + (e[2] + e[3]));
+            double c = s;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
                 const double up = __shfl_up(c, o);
                 if (lane >= o) c += up;
             }
-            const uint64_t over = __builtin_amdgcn_ballot_w64(e > 0.f && c > want);
-            const uint64_t any = __builtin_amdgcn_ballot_w64(e > 0.f);
-            if (over) found = base + __builtin_ctzll(over);
-            if (any) some = base + 63 - __builtin_clzll(any);
+            // this lane's first entry past `want`, and its last that holds any
+            double run = c - s;
+            int hit = -1, any = -1;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                run += (double)e[i];
+                if (!(e[i] > 0.f)) continue;
+                any = at + i;
+                if (hit < 0 && run > want) hit = at + i;
+            }
+            const uint64_t hits = __builtin_amdgcn_ballot_w64(hit >= 0), anys = __builtin_amdgcn_ballot_w64(any >= 0);
+            if (hits) found = __shfl(hit, __builtin_ctzll(hits));
+            if (anys) some = __shfl(any, 63 - __builtin_clzll(anys));
             want -= __shfl(c, 63);
         }
         if (lane == 0) {
             a.n_acc[blockIdx.x] = steps;
             // (rows that hold no probability: some token of the vocabulary)
-            a.next[blockIdx.x] = found >= 0 ? found : some >= 0 ? some : min(lo, V - 1);
+            a.next[blockIdx.x] = found >= 0 ? found : some >= 0 ? some : min(s0, V - 1);
         }
     }
     for (int i = tid; i < a.path_stride; i += kAccThreads)
