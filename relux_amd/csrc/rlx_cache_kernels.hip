@@ -253,14 +253,15 @@ hipError_t launch_mla_append(hipStream_t s, const PlanArg *plan, int tok_off, ui
 // grid.y = sequence of the call; x covers the sequence's work.  K: thread =
 // (token, head, 8-dim chunk), 16-byte read and write.  V: thread = (head, dim,
 // 8-token chunk), 16-byte read of a dim-major page row, 8 strided writes.
-__global__ void kv_gather_kernel(const uint16_t *__restrict__ kpool,
+template <bool ARG>
+__global__ void kv_gather_kernel(typename PlanSel<ARG>::T plan, const uint16_t *__restrict__ kpool,
                                  const uint16_t *__restrict__ vpool,
                                  const int32_t *__restrict__ table, const AttRow *__restrict__ rows,
                                  uint16_t *__restrict__ k_out, uint16_t *__restrict__ v_out,
                                  int kvh, int hd, int hdi, int P) {
     // Stored pages hold hd dims per head; the dense output holds the
     // caller's hdi (<= hd, a multiple of 8) and drops the zero padding.
-    const AttRow R = rows[blockIdx.y];
+    const AttRow R = plan_row<ARG>(rows, blockIdx.y);
     const int chunks = hdi >> 3;
     const int64_t nk = (int64_t)R.len * kvh * chunks;
     const int64_t base = (int64_t)R.qrow * kvh * hdi;  // qrow holds the output token offset
@@ -275,38 +276,48 @@ __global__ void kv_gather_kernel(const uint16_t *__restrict__ kpool,
         u32x4 v = *(const u32x4 *)(kpool + ((int64_t)page * kvh + h) * P * hd + k_page_off(slot, d0, hd));
         *(u32x4 *)(k_out + base + ((int64_t)h * R.len + t) * hdi + d0) = v;
     }
+    // V: 8 dims x 8 tokens a thread, turned in registers, neighbouring threads on
+    // neighbouring dims of the output rows.  16 sequences of 105 to 305 tokens, 8 kv
+    // heads of 128: 18.9 us by 2-byte stores.
     const int tchunks = (R.len + 7) >> 3;
-    const int64_t nv = (int64_t)kvh * hdi * tchunks;
+    const int64_t nv = (int64_t)kvh * tchunks * chunks;
     for (int64_t gid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; gid < nv;
          gid += (int64_t)gridDim.x * blockDim.x) {
-        const int tc = (int)(gid % tchunks);
-        const int hd_i = (int)(gid / tchunks);
-        const int h = hd_i / hdi;
-        const int d = hd_i - h * hdi;
-        const int t0 = tc * 8;
+        const int64_t ht = gid / chunks;
+        const int d0 = (int)(gid - ht * chunks) * 8, h = (int)(ht / tchunks), t0 = (int)(ht - (int64_t)h * tchunks) * 8;
         const int page = table[R.tab + t0 / P];
-        const int slot = t0 % P;
-        u32x4 v = *(const u32x4 *)(vpool + (((int64_t)page * kvh + h) * hd + d) * P + slot);
+        const uint16_t *src = vpool + (((int64_t)page * kvh + h) * hd + d0) * P + t0 % P;
+        u32x4 v[8];
+#pragma unroll
+        for (int d = 0; d < 8; d++) v[d] = *(const u32x4 *)(src + (int64_t)d * P);
+        uint16_t *dst = v_out + base + ((int64_t)h * R.len + t0) * hdi + d0;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            if (t0 + i < R.len) {
-                uint32_t w = v[i >> 1];
-                v_out[base + ((int64_t)h * R.len + t0 + i) * hdi + d] =
-                    (uint16_t)((i & 1) ? (w >> 16) : (w & 0xFFFFu));
+            if (t0 + i >= R.len) break;
+            u32x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t lo = v[2 * j][i >> 1] >> (16 * (i & 1)), hi = v[2 * j + 1][i >> 1] >> (16 * (i & 1));
+                w[j] = (lo & 0xFFFFu) | (hi << 16);
             }
+            *(u32x4 *)(dst + (int64_t)i * hdi) = w;
         }
     }
 }
 
-hipError_t launch_kv_gather(hipStream_t s, const uint16_t *kpool, const uint16_t *vpool,
+hipError_t launch_kv_gather(hipStream_t s, const PlanArg *plan, const uint16_t *kpool, const uint16_t *vpool,
                             const int32_t *table, const AttRow *rows, int n_rows, int max_len,
                             uint16_t *k_out, uint16_t *v_out, int kvh, int hd, int hdi, int P) {
     if (n_rows <= 0 || max_len <= 0) return hipSuccess;
     int64_t work = (int64_t)max_len * kvh * (hd / 8);
     int blocks = (int)((work + 255) / 256);
     if (blocks > 4096) blocks = 4096;
-    kv_gather_kernel<<<dim3(blocks, n_rows), 256, 0, s>>>(kpool, vpool, table, rows, k_out, v_out,
-                                                          kvh, hd, hdi, P);
+    if (plan)
+        kv_gather_kernel<true><<<dim3(blocks, n_rows), 256, 0, s>>>(*plan, kpool, vpool, table, rows, k_out, v_out, kvh,
+                                                                   hd, hdi, P);
+    else
+        kv_gather_kernel<false><<<dim3(blocks, n_rows), 256, 0, s>>>(NoPlan{0}, kpool, vpool, table, rows, k_out, v_out,
+                                                                    kvh, hd, hdi, P);
     return hipGetLastError();
 }
 

@@ -22,7 +22,6 @@
 #include <sys/mman.h>
 #include <unistd.h>
 
-#include <map>
 #include <new>
 #include <string>
 #include <vector>
@@ -102,6 +101,26 @@ struct LayerState {
     std::vector<SeqState> seqs;
 };
 
+// Table writes not yet on the device, in the order they were made; a later write of
+// an entry replaces an earlier one when they are taken.
+struct PendingWrites {
+    std::vector<Patch> w;
+    void set(int64_t idx, int32_t val) { w.push_back(Patch{(int32_t)idx, val}); }
+    bool empty() const { return w.empty(); }
+    void clear() { w.clear(); }
+    // The writes by index, each entry's last one.
+    std::vector<Patch> take() {
+        std::vector<Patch> p;
+        p.swap(w);
+        std::stable_sort(p.begin(), p.end(), [](const Patch &x, const Patch &y) { return x.idx < y.idx; });
+        size_t n = 0;
+        for (size_t i = 0; i < p.size(); i++)
+            if (i + 1 == p.size() || p[i + 1].idx != p[i].idx) p[n++] = p[i];
+        p.resize(n);
+        return p;
+    }
+};
+
 struct Slot {
     StagePair buf;
     hipEvent_t ev = nullptr;
@@ -138,7 +157,7 @@ struct Cache {
     std::vector<LayerState> L;
     int32_t *d_table = nullptr;
     hipStream_t own = nullptr, stream = nullptr;
-    std::map<int64_t, int32_t> pending;  // flat table index -> value
+    PendingWrites pending;
     Slot slots[kSlots];
     int next_slot = 0;
     Scratch ws;             // workspace
@@ -156,7 +175,7 @@ struct Cache {
     void set_entry(int layer, int seq, int k, int32_t v) {
         const int64_t idx = row_base(layer, seq) + k;
         L[layer].table[idx - (int64_t)layer * max_seqs * max_pages] = v;
-        pending[idx] = v;
+        pending.set(idx, v);
     }
     int32_t entry(int layer, int seq, int k) const {
         return L[layer].table[(int64_t)seq * max_pages + k];
@@ -269,13 +288,7 @@ struct Blob {
     }
 };
 
-std::vector<Patch> take_pending(Cache *c) {
-    std::vector<Patch> p;
-    p.reserve(c->pending.size());
-    for (auto &kv : c->pending) p.push_back(Patch{(int32_t)kv.first, kv.second});
-    c->pending.clear();
-    return p;
-}
+std::vector<Patch> take_pending(Cache *c) { return c->pending.take(); }
 
 // Apply pending table patches now (before a kernel that reads the table).
 int32_t flush_patches(Cache *c) {
@@ -293,17 +306,17 @@ int32_t flush_patches(Cache *c) {
 // Apply pending table patches through the kernel arguments (up to 256 per
 // launch): no staging slot, so nothing is allocated.
 int32_t flush_patches_inline(Cache *c) {
-    constexpr int kPer = kPlanArgBytes / (int)sizeof(Patch);
-    while (!c->pending.empty()) {
+    constexpr size_t kPer = kPlanArgBytes / sizeof(Patch);
+    const std::vector<Patch> p = c->pending.take();
+    for (size_t i = 0; i < p.size(); i += kPer) {
         PlanArg pa;
-        int n = 0;
-        auto it = c->pending.begin();
-        for (; it != c->pending.end() && n < kPer; ++it, ++n) {
-            const Patch p{(int32_t)it->first, it->second};
-            memcpy(pa.b + n * sizeof(Patch), &p, sizeof p);
+        const size_t n = std::min(kPer, p.size() - i);
+        memcpy(pa.b, p.data() + i, n * sizeof(Patch));
+        const hipError_t e = launch_patch_plan(c->stream, c->d_table, pa, (int)n);
+        if (e != hipSuccess) {  // what is not on its way stays pending
+            c->pending.w.assign(p.begin() + i, p.end());
+            HIP_TRY(e);
         }
-        HIP_TRY(launch_patch_plan(c->stream, c->d_table, pa, n));
-        c->pending.erase(c->pending.begin(), it);
     }
     return RLX_OK;
 }
@@ -514,19 +527,26 @@ int32_t plan_append(Cache *c, int layer, int n_seqs, const int32_t *seq_ids, con
         return fail(RLX_ERR_POOL, "page pool exhausted: layer %d needs %lld pages, %zu free", layer,
                     (long long)need_pages, ls.free_stack.size());
     int32_t row0 = 0;
+    size_t total = toks.size();
+    for (int i = 0; i < n_seqs; i++) total += n_tok[i];
+    toks.reserve(total);
     for (int i = 0; i < n_seqs; i++) {
         const int seq = seq_ids[i];
         SeqState &s = ls.seqs[seq];
+        int k = s.first + s.len / c->P, slot = s.len % c->P;
+        int32_t page = slot ? c->entry(layer, seq, k) : -1;
         for (int j = 0; j < n_tok[i]; j++) {
-            const int pos = s.len + j;
-            const int k = s.first + pos / c->P;
-            if (pos % c->P == 0) {
-                const int32_t page = ls.free_stack.back();
+            if (slot == 0) {
+                page = ls.free_stack.back();
                 ls.free_stack.pop_back();
                 c->set_entry(layer, seq, k, page);
                 s.pages++;
             }
-            toks.push_back(AppendTok{c->entry(layer, seq, k), pos % c->P, row0, n_tok[i]});
+            toks.push_back(AppendTok{page, slot, row0, n_tok[i]});
+            if (++slot == c->P) {
+                slot = 0;
+                k++;
+            }
         }
         s.len += n_tok[i];
         if (n_tok[i] > 0) s.chunks.push_back(n_tok[i]);
@@ -1531,14 +1551,17 @@ int32_t rlx_kv_gather(void *h, int32_t layer, int32_t n_seqs, const int32_t *seq
         ko = pad[0];
         vo = pad[1];
     }
-    Blob b;
-    size_t o_r = b.add(rows);
-    void *dev;
-    if ((rc = stage(c, b.bytes.data(), b.bytes.size(), &dev))) return rc;
+    // (rows in the kernel arguments where they fit)
+    PlanArg plan;
+    const bool args = rows.size() * sizeof(AttRow) <= sizeof plan;
+    void *dev = nullptr;
+    if (args)
+        memcpy(plan.b, rows.data(), rows.size() * sizeof(AttRow));
+    else if ((rc = stage(c, rows.data(), rows.size() * sizeof(AttRow), &dev)))
+        return rc;
     LayerState &ls = c->L[layer];
-    HIP_TRY(launch_kv_gather(c->stream, ls.pool0, ls.pool1, c->d_table,
-                             (const AttRow *)((char *)dev + o_r), n_seqs, max_len,
-                             (uint16_t *)ko, (uint16_t *)vo, c->kvh, c->hd, c->hdi, c->P));
+    HIP_TRY(launch_kv_gather(c->stream, args ? &plan : nullptr, ls.pool0, ls.pool1, c->d_table, (const AttRow *)dev,
+                             n_seqs, max_len, (uint16_t *)ko, (uint16_t *)vo, c->kvh, c->hd, c->hdi, c->P));
     if (pad_rows > 0) {
         HIP_TRY(launch_repack_rows(c->stream, ko, c->hdi, k_out, c->hdu, pad_rows, 2));
         HIP_TRY(launch_repack_rows(c->stream, vo, c->hdi, v_out, c->hdu, pad_rows, 2));

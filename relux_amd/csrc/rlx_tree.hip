@@ -918,37 +918,32 @@ __global__ __launch_bounds__(256) void tree_keep_kernel(PlanArg plan, const Keep
     kconst_i32 *way = (path ? (kconst_i32 *)(uintptr_t)path : (kconst_i32 *)(kernarg_plan() + path_off)) + p[7];
     __shared__ u32x4 sk[kTreeMaxNodes * 4];
     __shared__ uint16_t sv[kTreeMaxNodes * 32];
-    const int h = blockIdx.y, d0 = blockIdx.z * 32, w = min(32, hd - d0), kc = w / 8;
-    const auto page = [&](int node, int *slot) {
-        const int t = base + node, e = t / P;
-        *slot = t - e * P;
-        return ((int64_t)table[tab + e] * kvh + h) * P * hd;
-    };
-    for (int i = threadIdx.x; i < n * kc; i += 256) {
-        const int j = i / kc, c = i - j * kc;
-        int s;
-        const int64_t pb = page(way[j], &s);
-        sk[j * 4 + c] = *(const u32x4 *)(kpool + pb + k_page_off(s, d0 + c * 8, hd));
-    }
-    for (int i = threadIdx.x; i < n * w; i += 256) {
-        const int d = i / n, j = i - d * n;
-        int s;
-        const int64_t pb = page(way[j], &s);
-        sv[d * n + j] = vpool[pb + (int64_t)(d0 + d) * P + s];
+    __shared__ int64_t from[kTreeMaxNodes], to[kTreeMaxNodes];  // the head's page
+    __shared__ int from_slot[kTreeMaxNodes], to_slot[kTreeMaxNodes];
+    const int h = blockIdx.y, d0 = blockIdx.z * 32, w = min(32, hd - d0), t = threadIdx.x;
+    if (t < n) {
+        const auto page = [&](int node, int *slot) {
+            const int at = base + node, e = at / P;
+            *slot = at - e * P;
+            return ((int64_t)table[tab + e] * kvh + h) * P * hd;
+        };
+        from[t] = page(way[t], &from_slot[t]);
+        to[t] = page(t, &to_slot[t]);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n * kc; i += 256) {
-        const int j = i / kc, c = i - j * kc;
-        int s;
-        const int64_t pb = page(j, &s);
-        *(u32x4 *)(kpool + pb + k_page_off(s, d0 + c * 8, hd)) = sk[j * 4 + c];
-    }
-    for (int i = threadIdx.x; i < n * w; i += 256) {
-        const int d = i / n, j = i - d * n;
-        int s;
-        const int64_t pb = page(j, &s);
-        vpool[pb + (int64_t)(d0 + d) * P + s] = sv[d * n + j];
-    }
+    // K: a thread a node and 8 dims; V: a thread a node and dim
+    const int kj = t >> 2, kc = (t & 3) * 8, vj = t >> 5, vd = t & 31;
+    if (kc < w)
+        for (int j = kj; j < n; j += 64)
+            sk[j * 4 + (t & 3)] = *(const u32x4 *)(kpool + from[j] + k_page_off(from_slot[j], d0 + kc, hd));
+    if (vd < w)
+        for (int j = vj; j < n; j += 8) sv[j * 32 + vd] = vpool[from[j] + (int64_t)(d0 + vd) * P + from_slot[j]];
+    __syncthreads();
+    if (kc < w)
+        for (int j = kj; j < n; j += 64)
+            *(u32x4 *)(kpool + to[j] + k_page_off(to_slot[j], d0 + kc, hd)) = sk[j * 4 + (t & 3)];
+    if (vd < w)
+        for (int j = vj; j < n; j += 8) vpool[to[j] + (int64_t)(d0 + vd) * P + to_slot[j]] = sv[j * 32 + vd];
 }
 
 hipError_t launch_tree_keep(hipStream_t s, const PlanArg *plan, const KeepRow *rows, const int32_t *path, int path_off,
