@@ -249,10 +249,10 @@ class _PagedCache:
             raise TypeError("inv_freq must be a contiguous float32 vector on the cache's device")
         if 2 * inv_freq.numel() > head_dim:
             raise ValueError(f"{inv_freq.numel()} frequencies for {head_dim} dims")
-        check(self._lib.rlx_rope(self._h, rows, heads, head_dim, 2 * inv_freq.numel(), x.data_ptr(), _dtype_code(x),
-                                 x.stride(0), x.stride(1), _ints(positions, rows, "positions", self.device),
-                                 inv_freq.data_ptr(), float(scale), _PAIRING[layout], out.data_ptr(),
-                                 _dtype_code(out), out.stride(0), out.stride(1)))
+        pos, xt, ot = _ints(positions, rows, "positions", self.device), _dtype_code(x), _dtype_code(out)
+        check(self._lib.rlx_rope(self._h, rows, heads, head_dim, 2 * inv_freq.numel(), x.data_ptr(), xt, x.stride(0),
+                                 x.stride(1), pos, inv_freq.data_ptr(), float(scale), _PAIRING[layout],
+                                 out.data_ptr(), ot, out.stride(0), out.stride(1)))
         return out
 
     def _lens(self, layer_idx, seq_ids):
@@ -449,10 +449,11 @@ class KVCache(_PagedCache):
         for t, what in ((q, "q"), (out, "out")):
             if t.device != self.device:
                 raise TypeError(f"{what} must be a tensor on {self.device}")
+        up = _ints(parents, sum(n_nodes), "parents", self.device)
+        qp, qt, op, ot = _dev(q, "q"), _dtype_code(q), _dev(out, "out"), _dtype_code(out)
         check(self._lib.rlx_gqa_attend_tree(
-            self._h, layer_idx, len(seq_ids), i32_array(seq_ids), i32_array(n_nodes), i32_array(n_q), num_heads,
-            _dev(q, "q"), _dtype_code(q), _LAYOUTS[layout], float(scale or 0.0),
-            _ints(parents, sum(n_nodes), "parents", self.device), _dev(out, "out"), _dtype_code(out)))
+            self._h, layer_idx, len(seq_ids), i32_array(seq_ids), i32_array(n_nodes), i32_array(n_q), num_heads, qp, qt,
+            _LAYOUTS[layout], float(scale or 0.0), up, op, ot))
         return out
 
     def KeepPath(self, seq, n_nodes, path, layer=-1):
