@@ -51,15 +51,52 @@ __device__ __forceinline__ float4 acc_load4(const float *row, int i, int end, bo
 // Weight of a logit: exp2(l k - m k), mk = m k rounded once for the whole row.
 __device__ __forceinline__ float acc_e(float l, float k, float mk) { return __builtin_amdgcn_exp2f(fmaf(l, k, -mk)); }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+// v of the lane that a row move (16 lanes) takes; 0 where it takes none or the row is masked.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ float row_move(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xF, false));
 }
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double row_move(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false),
+                   hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {  // lane: the same in every lane
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+constexpr int kRor = 0x120, kShr = 0x110, kBcast15 = 0x142, kBcast31 = 0x143;  // rotate and shift within a row; a row's last lane to later ones
+
+// Over the 16 lanes of a row, the same in each.
+__device__ __forceinline__ double row_sum(double v) {
+    v += row_move<kRor + 8>(v);
+    v += row_move<kRor + 4>(v);
+    v += row_move<kRor + 2>(v);
+    return v + row_move<kRor + 1>(v);
+}
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, row_move<kRor + 8>(v));
+    v = fmaxf(v, row_move<kRor + 4>(v));
+    v = fmaxf(v, row_move<kRor + 2>(v));
+    return fmaxf(v, row_move<kRor + 1>(v));
+}
+// Over the wave.
+__device__ __forceinline__ double wave_sum(double v) {
+    v = row_sum(v);
+    return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+__device__ __forceinline__ float wave_max(float v) { return rows4_max(row_max(v)); }
+// Sums of lanes 0 .. lane.
+__device__ __forceinline__ double wave_scan(double v) {
+    v += row_move<kShr + 1>(v);
+    v += row_move<kShr + 2>(v);
+    v += row_move<kShr + 4>(v);
+    v += row_move<kShr + 8>(v);
+    v += row_move<kBcast15, 0xA>(v);
+    return v + row_move<kBcast31, 0xC>(v);
 }
 
 constexpr int kAccBatch = 4;  // float4 of a row a lane has in flight
@@ -100,8 +137,8 @@ template <bool Q>
 __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, TreeAcceptArgs a) {
     __shared__ int par[kTreeMaxNodes], tok[kTreeMaxNodes], gone[kTreeMaxNodes], way[kTreeMaxNodes];
     __shared__ float uni[kTreeMaxNodes], lt[kTreeMaxNodes], lq[kTreeMaxNodes];
-    __shared__ float red_m[2][kAccWaves];
-    __shared__ double red_s[2][kAccWaves], part[2][kAccWaves];  // part: the waves' sums, two passes in turn
+    __shared__ float red_m[2][2][kAccWaves];  // the waves' sums, two passes in turn: one barrier a pass
+    __shared__ double red_s[2][2][kAccWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int first, n;
     {
@@ -111,12 +148,14 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
     }
     const int V = a.V;
     const float k = 1.4426950408889634f / a.temperature;
+    // (used when the root's rows have been read)
+    int my_par = 0, my_tok = 0;
+    float my_u = 0.f;
     if (tid < n) {
-        par[tid] = a.parents[first + tid];
-        tok[tid] = a.tok[first + tid];
-        uni[tid] = a.u[first + tid];
+        my_par = a.parents[first + tid];
+        my_tok = a.tok[first + tid];
+        my_u = a.u[first + tid];
     }
-    __syncthreads();
 
     // Wave w covers entries [w * span, (w + 1) * span) of a row, 256 at a time.
     const int span = (V + kAccWaves * 256 - 1) / (kAccWaves * 256) * 256;
@@ -168,16 +207,15 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
         return s;
     };
     int turn = 0;
-    // Sum over the row; the waves' sums stay in part[turn].
+    double waves;  // lane w of a row: what remains in wave w's span
+    // Sum of what remains over the row.
     auto total = [&]() {
         const double s = wave_sum(mass(v0, v1));
         turn ^= 1;
-        if (lane == 0) part[turn][wave] = s;
+        if (lane == 0) red_s[turn][0][wave] = s;
         __syncthreads();
-        double z = 0.0;
-#pragma unroll
-        for (int w = 0; w < kAccWaves; w++) z += part[turn][w];
-        return z;
+        waves = red_s[turn][0][lane & 15];
+        return row_sum(waves);
     };
 
     for (;;) {
@@ -185,49 +223,67 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
         d = Q ? a.d_logits + (int64_t)(first + cur) * a.d_stride : nullptr;
         // this node's children, and their logits
         uint64_t kids[kTreeMaxNodes / 64];
+        float my_t = 0.f, my_d = 0.f;
+        bool mine = false;
+        auto children = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int w = 0; w < kTreeMaxNodes / 64; w++) {
-            const int j = w * 64 + lane;
-            kids[w] = __builtin_amdgcn_ballot_w64(j > cur && j < n && par[j] == cur);
-        }
-        if (tid > cur && tid < n && par[tid] == cur && tok[tid] >= 0 && tok[tid] < V) {
-            lt[tid] = t[tok[tid]];
-            if (Q) lq[tid] = d[tok[tid]];
-        }
-        // the rows' masses (the draft's only where there are children)
-        const bool parent = Q && (kids[0] | kids[1] | kids[2] | kids[3]);
-        {
-            Online ot, oq;
-            for (int base = v0; base < v1; base += kAccBatch * 256) {
-                float4 x[kAccBatch], y[kAccBatch];
-                load(t, x, base, v1);
-                if (parent) load(d, y, base, v1);
-                ot.add(x, k, base == v0);
-                if (parent) oq.add(y, k, base == v0);
+            for (int w = 0; w < kTreeMaxNodes / 64; w++) {
+                const int j = w * 64 + lane;
+                kids[w] = __builtin_amdgcn_ballot_w64(j > cur && j < n && par[j] == cur);
             }
-            auto fold = [&](Online &o, int side) {
-                const double z = wave_sum(o.s);
-                if (lane == 0) {
-                    red_m[side][wave] = v0 < v1 ? o.mk : -INFINITY;
-                    red_s[side][wave] = z;
-                }
-            };
-            fold(ot, 0);
-            if (parent) fold(oq, 1);
+            mine = tid > cur && tid < n && par[tid] == cur && tok[tid] >= 0 && tok[tid] < V;
+            if (mine) {
+                my_t = t[tok[tid]];
+                if (Q) my_d = d[tok[tid]];
+            }
+        };
+        // the rows' masses (the draft's only where there are children)
+        bool parent = Q && n > 1;
+        if (steps > 0) {
+            children();
+            parent = Q && (kids[0] | kids[1] | kids[2] | kids[3]);
+        }
+        Online ot, oq;
+        for (int base = v0; base < v1; base += kAccBatch * 256) {
+            float4 x[kAccBatch], y[kAccBatch];
+            load(t, x, base, v1);
+            if (parent) load(d, y, base, v1);
+            ot.add(x, k, base == v0);
+            if (parent) oq.add(y, k, base == v0);
+        }
+        turn ^= 1;
+        auto fold = [&](Online &o, int side) {
+            const double z = wave_sum(o.s);
+            if (lane == 0) {
+                red_m[turn][side][wave] = v0 < v1 ? o.mk : -INFINITY;
+                red_s[turn][side][wave] = z;
+            }
+        };
+        fold(ot, 0);
+        if (parent) fold(oq, 1);
+        if (steps == 0) {
+            if (tid < n) {
+                par[tid] = my_par;
+                tok[tid] = my_tok;
+                uni[tid] = my_u;
+            }
             __syncthreads();
-            auto join = [&](int side) {
-                RowStat r{-INFINITY, 0.0};
-#pragma unroll
-                for (int w = 0; w < kAccWaves; w++) r.mk = fmaxf(r.mk, red_m[side][w]);
-#pragma unroll
-                for (int w = 0; w < kAccWaves; w++) r.z += red_s[side][w] * (double)__builtin_amdgcn_exp2f(red_m[side][w] - r.mk);
-                return r;
-            };
-            T = join(0);
-            if (parent) D = join(1);
-            turn ^= 1;
-            if (tid < kAccWaves) part[turn][tid] = red_s[0][tid] * (double)__builtin_amdgcn_exp2f(red_m[0][tid] - T.mk);
-            __syncthreads();
+            children();
+        }
+        if (mine) {
+            lt[tid] = my_t;
+            if (Q) lq[tid] = my_d;
+        }
+        __syncthreads();
+        auto join = [&](int side, double &each) {
+            const float m = red_m[turn][side][lane & 15], mk = row_max(m);
+            each = red_s[turn][side][lane & 15] * (double)__builtin_amdgcn_exp2f(m - mk);
+            return RowStat{mk, row_sum(each)};
+        };
+        T = join(0, waves);
+        if (parent) {
+            double each;
+            D = join(1, each);
         }
         C = 0.0;
         S = 1.0;
@@ -253,6 +309,8 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
                         went = c;
                         break;
                     }
+                    if (tid == 0) gone[n_gone] = x;
+                    n_gone++;
                     if (S > 0.0) {
                         C += A / T.z / S;
                         S -= qx;
@@ -263,6 +321,8 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
                             ratio = 0.f;
                             A = total();
                         }
+                    } else {
+                        __syncthreads();
                     }
                 } else {
                     if ((double)uni[c] * A < (double)et) {
@@ -270,49 +330,42 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
                         break;
                     }
                     A -= (double)et;
+                    if (tid == 0) gone[n_gone] = x;
+                    n_gone++;
+                    __syncthreads();
                 }
-                __syncthreads();
-                if (tid == 0) gone[n_gone] = x;
-                n_gone++;
-                __syncthreads();
             }
         }
         if (went < 0) break;
         cur = went;
         steps++;
         if (tid == 0) way[steps] = cur;
-        __syncthreads();
     }
 
     // ---- the next token: the first whose cumulated mass exceeds u A --------------
     if (!Q && n_gone) A = total();
     double want = (double)uni[0] * A;
-    // Which of the waves' sums `want` falls in (else the last that holds any); want
-    // becomes what is left of it there.
-    auto pick = [&](const double *sums) {
-        const double s = lane < kAccWaves ? fmax(sums[lane], 0.0) : 0.0;
-        double c = s;
-#pragma unroll
-        for (int o = 1; o < kAccWaves; o <<= 1) {
-            const double up = __shfl_up(c, o);
-            if (lane >= o) c += up;
-        }
+    // Which of `waves` `want` falls in (else the last that holds any); want becomes
+    // what is left of it there.
+    auto pick = [&]() {
+        const double s = lane < kAccWaves ? fmax(waves, 0.0) : 0.0, c = wave_scan(s);
         const uint64_t any = __builtin_amdgcn_ballot_w64(s > 0.0), over = __builtin_amdgcn_ballot_w64(s > 0.0 && c > want);
         const int w = over ? __builtin_ctzll(over) : any ? 63 - __builtin_clzll(any) : 0;
-        want -= __shfl(c - s, w);
+        want -= lane_of(c - s, w);
         return w;
     };
     // the wave's span again by all the waves, then a part of it by one
-    int lo = pick(part[turn]) * span;
+    int lo = pick() * span;
     const int sub = span / kAccWaves, hi = min(V, lo + span);
     const int s0 = min(hi, lo + wave * sub), s1 = min(hi, s0 + sub);
     {
         const double s = wave_sum(mass(s0, s1));
         turn ^= 1;
-        if (lane == 0) part[turn][wave] = s;
+        if (lane == 0) red_s[turn][0][wave] = s;
     }
     __syncthreads();
-    const int owner = pick(part[turn]);
+    waves = red_s[turn][0][lane & 15];
+    const int owner = pick();
     if (wave == owner) {
         int found = -1, some = -1;
         for (int base = s0; base < s1 && found < 0; base += 256) {
@@ -331,13 +384,7 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
 #pragma unroll
                 for (int c = 0; c < 4; c++)
                     if (gone[g] == at + c) e[c] = 0.f;
-            const double s = (double)((e[0] + e[1]) + (e[2] + e[3]));
-            double c = s;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double up = __shfl_up(c, o);
-                if (lane >= o) c += up;
-            }
+            const double s = (double)((e[0] + e[1]) + (e[2] + e[3])), c = wave_scan(s);
             // this lane's first entry past `want`, and its last that holds any
             double run = c - s;
             int hit = -1, any = -1;
@@ -349,9 +396,9 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
                 if (hit < 0 && run > want) hit = at + i;
             }
             const uint64_t hits = __builtin_amdgcn_ballot_w64(hit >= 0), anys = __builtin_amdgcn_ballot_w64(any >= 0);
-            if (hits) found = __shfl(hit, __builtin_ctzll(hits));
-            if (anys) some = __shfl(any, 63 - __builtin_clzll(anys));
-            want -= __shfl(c, 63);
+            if (hits) found = __builtin_amdgcn_readlane(hit, __builtin_ctzll(hits));
+            if (anys) some = __builtin_amdgcn_readlane(any, 63 - __builtin_clzll(anys));
+            want -= lane_of(c, 63);
         }
         if (lane == 0) {
             a.n_acc[blockIdx.x] = steps;
