@@ -102,16 +102,18 @@ __device__ __forceinline__ double wave_scan(double v) {
 constexpr int kAccBatch = 4;  // float4 of a row a lane has in flight
 
 // A wave's sum of exp2(l k - mk), mk of the wave's first batch's maximum unless a
-// later entry exceeds it by 2^60.
+// later entry exceeds it by 2^60.  kNone: only -inf so far, below any other maximum
+// and finite, so that -inf - mk is -inf.
+constexpr float kNone = -3e38f;
 struct Online {
-    float mk = 0.f;
+    float mk = kNone;
     double s = 0.0;  // this lane's
     __device__ __forceinline__ void add(const float4 (&v)[kAccBatch], float k, bool first) {
         float x = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kAccBatch; i++) x = fmaxf(x, fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i].z, v[i].w)));
         if (first || __builtin_amdgcn_ballot_w64(x * k > mk + 60.f)) {
-            const float m = wave_max(x) * k, to = m == -INFINITY ? 0.f : m;
+            const float to = fmaxf(wave_max(x) * k, kNone);
             if (!first) s *= (double)__builtin_amdgcn_exp2f(mk - to);
             mk = to;
         }
@@ -255,7 +257,7 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
         auto fold = [&](Online &o, int side) {
             const double z = wave_sum(o.s);
             if (lane == 0) {
-                red_m[turn][side][wave] = v0 < v1 ? o.mk : -INFINITY;
+                red_m[turn][side][wave] = o.mk;
                 red_s[turn][side][wave] = z;
             }
         };

@@ -389,6 +389,21 @@ def test_tree_accept_edges(gpu):
         assert 0 <= nxt[0] < V
 
 
+@pytest.mark.parametrize("draft", [True, False])
+@pytest.mark.parametrize("mask", [-np.inf, np.finfo(np.float32).min])
+def test_tree_accept_few_tokens_far_below_zero(gpu, mask, draft):
+    """Rows of masked entries but for a few, whose logits lie hundreds below zero."""
+    V, gen = 20000, np.random.default_rng(21)
+    live = np.array([3, 4, 5, 4940, 4941, 9999, 19990, 19999])
+    for trial in range(20):
+        t, d = (np.full((9, V), mask, np.float32) for _ in range(2))
+        t[:, live] = gen.standard_normal((9, 8)) - 700
+        d[:, live] = t[:, live] + 0.5 * gen.standard_normal((9, 8))
+        tok = gen.choice(live, 9).astype(np.int32)
+        case = ([9], [[-1, 0, 0, 0, 1, 1, 2, 4, 4]], t, d if draft else None, tok, gen.random(9, dtype=np.float32))
+        assert _accept(gpu, *case, 1.0) == _want(*case, 1.0)
+
+
 def test_tree_accept_strided_rows_and_guards(gpu):
     from relux_amd import Sampler, tree_accept_async
     sizes, trees, t, d, tok, u = _drafts(5, 333, (3, 20), 1.0, True, 77, gpu)
