@@ -99,6 +99,9 @@ __device__ __forceinline__ double wave_scan(double v) {
     return v + row_move<kBcast31, 0xC>(v);
 }
 
+// A condition that is the same in every lane, as a scalar one.
+__device__ __forceinline__ bool same(bool c) { return __builtin_amdgcn_ballot_w64(c) != 0; }
+
 constexpr int kAccBatch = 4;  // float4 of a row a lane has in flight
 
 // A wave's sum of exp2(l k - mk), mk of the wave's first batch's maximum unless a
@@ -167,6 +170,7 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
     const float *t, *d;
     RowStat T{0.f, 0.0}, D{0.f, 1.0};
     double C, S, A;  // A in units of the target's weights (p's mass = T.z)
+    bool subtract = false;  // ratio > 0
     float ratio;     // C in those units: max(0, e_t - ratio e_q)
     auto rest = [&](float et, float eq) __attribute__((always_inline)) {
         return Q ? fmaxf(0.f, fmaf(-ratio, eq, et)) : et;
@@ -183,12 +187,12 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
         for (int base = lo; base < hi; base += kAccBatch * 256) {
             float4 x[kAccBatch], y[kAccBatch];
             load(t, x, base, hi);
-            if (Q && ratio > 0.f) load(d, y, base, hi);
+            if (Q && subtract) load(d, y, base, hi);
             float sum[kAccBatch];
 #pragma unroll
             for (int i = 0; i < kAccBatch; i++) {
                 float e[4] = {acc_e(x[i].x, k, T.mk), acc_e(x[i].y, k, T.mk), acc_e(x[i].z, k, T.mk), acc_e(x[i].w, k, T.mk)};
-                if (Q && ratio > 0.f) {
+                if (Q && subtract) {
                     e[0] = rest(e[0], acc_e(y[i].x, k, D.mk));
                     e[1] = rest(e[1], acc_e(y[i].y, k, D.mk));
                     e[2] = rest(e[2], acc_e(y[i].z, k, D.mk));
@@ -291,6 +295,7 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
         S = 1.0;
         A = T.z;
         ratio = 0.f;
+        subtract = false;
         n_gone = 0;
         int went = -1;
 #pragma unroll 1
@@ -299,35 +304,37 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
             while (left) {
                 const int c = w * 64 + __builtin_ctzll(left);
                 left &= left - 1;
-                const int x = tok[c];
+                const int x = __builtin_amdgcn_readfirstlane(tok[c]);
                 bool skip = x < 0 || x >= V;  // no token: rejected without effect, as a rejected token again is
-                for (int g = 0; g < n_gone; g++) skip |= gone[g] == x;
-                if (skip) continue;
+                for (int g = lane; g < n_gone; g += 64) skip |= gone[g] == x;
+                if (same(skip)) continue;
                 const float et = acc_e(lt[c], k, T.mk);
                 if constexpr (Q) {
                     const float eq = acc_e(lq[c], k, D.mk);
                     const double qx = (double)eq / D.z, px = (double)rest(et, eq);
-                    if (S > 0.0 ? (double)uni[c] * qx * A < px * S : px > 0.0) {
+                    if (same(S > 0.0 ? (double)uni[c] * qx * A < px * S : px > 0.0)) {
                         went = c;
                         break;
                     }
                     if (tid == 0) gone[n_gone] = x;
                     n_gone++;
-                    if (S > 0.0) {
+                    if (same(S > 0.0)) {
                         C += A / T.z / S;
                         S -= qx;
                         ratio = (float)fmin(C * T.z / D.z, 3e38);  // (finite: 0 where a draft weight is 0)
+                        subtract = true;
                         A = total();
-                        if (!(A > 0.0)) {  // nothing is left by rounding alone
+                        if (same(!(A > 0.0))) {  // nothing is left by rounding alone
                             C = 0.0;
                             ratio = 0.f;
+                            subtract = false;
                             A = total();
                         }
                     } else {
                         __syncthreads();
                     }
                 } else {
-                    if ((double)uni[c] * A < (double)et) {
+                    if (same((double)uni[c] * A < (double)et)) {
                         went = c;
                         break;
                     }
@@ -375,7 +382,7 @@ __global__ __launch_bounds__(kAccThreads) void tree_accept_kernel(PlanArg plan, 
             const bool full = base + 256 <= s1;
             const float4 x = acc_load4(t, at, s1, full);
             float e[4] = {acc_e(x.x, k, T.mk), acc_e(x.y, k, T.mk), acc_e(x.z, k, T.mk), acc_e(x.w, k, T.mk)};
-            if (Q && ratio > 0.f) {
+            if (Q && subtract) {
                 const float4 y = acc_load4(d, at, s1, full);
                 e[0] = rest(e[0], acc_e(y.x, k, D.mk));
                 e[1] = rest(e[1], acc_e(y.y, k, D.mk));
