@@ -3313,30 +3313,22 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
     const std::vector<int> &cuts = tp.cuts;
     const int qt = tp.tile;
     const auto tiles = [&](int i) { return (load[i].rows + qt - 1) / qt; };
-    int64_t wgs = 0, parts = 0, n_cuts = 0;
-    int max_tiles = 1;
+    int64_t wgs = 0, parts = 0;
     bool merge = false;
     // the longest cuts first, so that the last round is of short ones
     std::vector<int> order(n_seqs);
-    for (int i = 0; i < n_seqs; i++) {
-        order[i] = i;
-        n_cuts += cuts[i];
-        max_tiles = std::max(max_tiles, tiles(i));
-    }
+    for (int i = 0; i < n_seqs; i++) order[i] = i;
     std::stable_sort(order.begin(), order.end(), [&](int x, int y) {
         return (int64_t)load[x].len * cuts[y] > (int64_t)load[y].len * cuts[x];
     });
-    const bool spread = n_cuts >= 16;
     std::vector<TreeRow> by_cut(n_seqs);
-    int at = 0;
     for (int k = 0; k < n_seqs; k++) {
         const int i = order[k];
         const int64_t n = (int64_t)tiles(i) * c->kvh * cuts[i];
         by_cut[k] = rows[i];
         by_cut[k].nsplit = cuts[i];
-        by_cut[k].at0 = spread ? at : (int32_t)wgs;
+        by_cut[k].wg0 = (int32_t)wgs;
         by_cut[k].part = (int32_t)parts;
-        at += cuts[i];
         wgs += n;
         if (cuts[i] > 1) {
             parts += n;
@@ -3344,7 +3336,6 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
         }
     }
     rows.swap(by_cut);
-    if (spread) wgs = (n_cuts + 7) / 8 * 8 * c->kvh * max_tiles;
     if (wgs > 0x7FFFFFFF) return fail(RLX_ERR_UNSUPPORTED, "rlx_gqa_attend_tree: %lld work-groups", (long long)wgs);
     int32_t rc;
     if ((rc = flush_patches(c))) return rc;
@@ -3358,7 +3349,7 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
         std::vector<int32_t> work;
         for (int k = 0; k < n_seqs; k++) {
             const int i = order[k];
-            work.insert(work.end(), spread ? cuts[i] : tiles(i) * c->kvh * cuts[i], k);
+            work.insert(work.end(), (size_t)tiles(i) * c->kvh * cuts[i], k);
         }
         Blob b;
         const size_t o_r = b.add(rows), o_w = b.add(work);
@@ -3384,9 +3375,6 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
     a.q_bf16 = q_dtype == RLX_BF16;
     a.out_bf16 = out_dtype == RLX_BF16;
     a.layout = qo_layout;
-    a.spread = spread;
-    a.n_at = (int)n_cuts;
-    a.max_tiles = max_tiles;
     if (!(scale > 0.f)) scale = (float)(1.0 / std::sqrt((double)c->hdu));
     a.qscale = scale * 1.4426950408889634f;
     hipEvent_t e0, e1;

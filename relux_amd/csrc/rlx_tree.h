@@ -16,7 +16,7 @@ struct TreeRow {
     int32_t qrow;    // first call-row of this sequence's queries / outputs
     int32_t node0;   // first entry of this sequence in `parents`
     int32_t nsplit;  // cuts along the keys
-    int32_t at0;     // first work-group (TreeArgs::spread: first cut)
+    int32_t wg0;     // first work-group
     int32_t part;    // first partial slot (nsplit > 1)
 };
 static_assert(sizeof(TreeRow) == 32, "TreeRow is 8 int32");
@@ -25,15 +25,14 @@ struct TreeArgs {
     const uint16_t *kpool, *vpool;
     const int32_t *table;
     const TreeRow *rows;     // device rows, or nullptr: in the plan argument
-    const int32_t *work;     // device rows only: the row of each work-group (spread: of each cut)
+    const int32_t *work;     // device rows only: the row of each work-group
     const int32_t *parents;
     const void *q;
     void *out;
     float *part_o, *part_ml;  // [slot][rows of a tile][D], [slot][rows of a tile][max, sum]
     int n_rows, H, KVH, DQ, P, pshift;  // pshift: log2(P), or -1
     int q_bf16, out_bf16, layout;
-    int spread, n_at, max_tiles;  // cuts dealt out over the XCDs: their number, and the most tiles of a row
-    float qscale;                 // scale * log2(e)
+    float qscale;  // scale * log2(e)
 };
 
 // fine: queries and weights in parts of bf16, for f32 queries or outputs.

@@ -90,32 +90,21 @@ struct TreeItem {
     TreeRow R;
     int nodes, nq, G, QR, tiles, split, kvh, tile, ctx, u0, u1;  // ctx: first key of the tree; u: units of 32 keys
 };
-// The item of work-group blockIdx.x; false: none.
+// The item of work-group blockIdx.x.
 //
-// Work-group b runs on XCD b mod 8, each with its own L2 and address translation.
-// With cuts enough (a.spread) the cuts of all sequences, end to end, are dealt
-// out over the XCDs and a cut's kv heads and tiles run on one: they read the same
-// pages, 4 KB apart, and tiles the same keys.  The 16 x 8192 token call: .... With
-// few cuts that would leave XCDs idle: a row's cuts and kv heads are dealt out, a
-// pair's tiles 8 apart.
+// Work-group b runs on XCD b mod 8, each with its own L2: the tiles of a (cut, kv
+// head) pair read the same keys and are put 8 apart, the pairs dealt out.
 template <int QT>
-__device__ __forceinline__ bool tree_item(const TreeArgs &a, TreeItem &w) {
+__device__ __forceinline__ void tree_item(const TreeArgs &a, TreeItem &w) {
     const int b = blockIdx.x;
-    int at = b, i = 0;  // what the rows are searched by; the item within a cut
-    if (a.spread) {
-        const int per = a.KVH * a.max_tiles, y = b >> 3;
-        at = y / per * 8 + (b & 7);
-        i = y % per;
-        if (at >= a.n_at) return false;
-    }
     int r;
     if (a.rows) {
-        r = ((kconst_i32 *)(uintptr_t)a.work)[at];
+        r = ((kconst_i32 *)(uintptr_t)a.work)[b];
     } else {
         int lo = 0, hi = a.n_rows - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (plan_ints(nullptr, mid, 8)[6] <= at)
+            if (plan_ints(nullptr, mid, 8)[6] <= b)
                 lo = mid;
             else
                 hi = mid - 1;
@@ -128,25 +117,16 @@ __device__ __forceinline__ bool tree_item(const TreeArgs &a, TreeItem &w) {
     w.G = a.H / a.KVH;
     w.QR = w.nq * w.G;
     w.tiles = (w.QR + QT - 1) / QT;
-    if (a.spread) {
-        w.split = at - w.R.at0;
-        w.kvh = i / a.max_tiles;
-        w.tile = i - w.kvh * a.max_tiles;
-        if (w.tile >= w.tiles) return false;
-    } else {
-        const int streams = w.R.nsplit * a.KVH;
-        i = b - w.R.at0;
-        const int s0 = i / (8 * w.tiles) * 8, m = min(8, streams - s0), rem = i - s0 * w.tiles;
-        w.tile = rem / m;
-        const int stream = s0 + rem - w.tile * m;
-        w.split = stream / a.KVH;
-        w.kvh = stream - w.split * a.KVH;
-    }
+    const int pairs = w.R.nsplit * a.KVH, i = b - w.R.wg0;
+    const int s0 = i / (8 * w.tiles) * 8, m = min(8, pairs - s0), rem = i - s0 * w.tiles;
+    w.tile = rem / m;
+    const int pair = s0 + rem - w.tile * m;
+    w.split = pair / a.KVH;
+    w.kvh = pair - w.split * a.KVH;
     w.ctx = w.R.len - w.nodes;
     const int units = (w.R.len + kTreeKeys - 1) / kTreeKeys;
     w.u0 = (int)((int64_t)w.split * units / w.R.nsplit);
     w.u1 = (int)((int64_t)(w.split + 1) * units / w.R.nsplit);
-    return true;
 }
 // Partial slot of (cut, kv head, tile) of a row.
 __device__ __forceinline__ int64_t tree_slot(const TreeRow &R, int KVH, int tiles, int split, int kvh, int tile) {
@@ -508,7 +488,10 @@ struct TreeLane {
 
 // Few query rows: 4 waves, each holding all 16 NQT rows of the tile and taking
 // every fourth unit, straight from HBM into registers in the operands' order -- no
-// LDS and no barrier in the loop.  HBM-bound.
+// LDS and no barrier in the loop.  HBM-bound: 16 sequences of 8192 tokens, 16 nodes,
+// 32 / 8 heads of 128, bf16, 99 us, 5.4 TB/s (a large copy moves 5.2).  One of 200
+// tokens, 7 nodes, f32: 12 us, a launch and the chain of reads (plan, table, keys),
+// products and joins of its one round.
 // SHARED: other tiles read the same keys, which stay in L2 (else non-temporal loads).
 template <int D, int NQT, bool FINE, bool SHARED>
 __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeArgs a) {
@@ -521,7 +504,7 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
     __shared__ fl4 so[4][MC][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TreeItem w;
-    if (!tree_item<QT>(a, w)) return;
+    tree_item<QT>(a, w);
     const int parent = threadIdx.x < w.nodes ? a.parents[w.R.node0 + threadIdx.x] : -1;
 
     const int first = w.u0 + wave, nu = first < w.u1 ? (w.u1 - first + 3) / 4 : 0;
@@ -662,7 +645,9 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
 // fragment at 16 lane: reads without bank conflicts).  A wave takes the scores of unit
 // u + 1 while it turns those of unit u into weights, so that the matrix unit works
 // through the softmax; two waves a SIMD hide the rest.  HBM-bound at few rows, by
-// the matrix and softmax units at many.
+// the matrix and softmax units at many: 24 sequences of 1000 to 12000 tokens, 40 to
+// 64 nodes, 64 / 8 heads of 128, bf16: 257 us with the merge's 20, 690 TFLOP/s (a large
+// library product reaches 1200), matrix units 36 % busy.
 template <int D, int NQT, int WAVES, bool FINE>
 __global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void tree_wide_kernel(PlanArg plan, TreeArgs a) {
     using W = TreeWave<D, NQT, FINE, (D > 128 && WAVES == 4)>;
@@ -678,7 +663,7 @@ __global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void t
     __shared__ u32x4 ring[STAGES * UPS][UNIT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     TreeItem w;
-    if (!tree_item<QT>(a, w)) return;
+    tree_item<QT>(a, w);
     const int parent = threadIdx.x < w.nodes ? a.parents[w.R.node0 + threadIdx.x] : -1;
 
     const int nu = w.u1 - w.u0;
@@ -810,7 +795,7 @@ __global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void t
 }
 
 // Joins the partials of the sequences whose keys were cut: a thread holds 4 dims
-// of a query row.  out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.
+// of a query row.  out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  HBM-bound.
 __global__ __launch_bounds__(256) void tree_merge_kernel(PlanArg plan, TreeArgs a, int D, int QT) {
     const TreeRow R = tree_row(a.rows, blockIdx.x);
     if (R.nsplit <= 1) return;
@@ -907,7 +892,8 @@ hipError_t launch_tree_attend(hipStream_t s, const PlanArg &plan, const TreeArgs
 // Moves the accepted nodes' K and V rows of (layer, sequence) blockIdx.x, kv head
 // blockIdx.y, dims [32 blockIdx.z, + 32): node path[j] to the tree's slot j, every
 // row read before the first is written (a slot may be both).  Latency-bound: 64 bytes of K
-// and 32 2-byte elements of V a node.
+// and 32 2-byte elements of V a node.  16 layers of 16 sequences of 24 to 48 nodes, 8 kv
+// heads of 128: 19 us.
 __global__ __launch_bounds__(256) void tree_keep_kernel(PlanArg plan, const KeepRow *rows, const int32_t *path,
                                                         int path_off, const int32_t *__restrict__ table, int kvh,
                                                         int hd, int P) {
