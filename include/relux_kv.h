@@ -406,8 +406,9 @@ int32_t rlx_rope(void *cache, int64_t rows, int32_t heads, int32_t head_dim, int
  * ancestors.  A parent outside [0, node) ends the chain (a root).  Values of
  * nodes a query does not attend do not reach it, infinities and NaN included.
  * q, out and the rest as for rlx_gqa_attend, but out must not overlap q.  f32
- * queries, or f32 outputs, are computed to about 2^-17; bf16 both ways rounds
- * the softmax weights to bf16. */
+ * queries, or f32 outputs, are computed as exactly as f32; bf16 both ways rounds
+ * the softmax weights to bf16.  A call whose keys are cut takes workspace for its
+ * partial sums (see rlx_cache_reserve). */
 int32_t rlx_gqa_attend_tree(void *cache, int32_t layer, int32_t n_seqs, const int32_t *seq_ids,
                             const int32_t *n_nodes, const int32_t *n_q, int32_t num_heads,
                             const void *q, int32_t q_dtype, int32_t qo_layout, float scale,

@@ -646,7 +646,7 @@ __global__ __launch_bounds__(256, 1) void tree_narrow_kernel(PlanArg plan, TreeA
 // u + 1 while it turns those of unit u into weights, so that the matrix unit works
 // through the softmax; two waves a SIMD hide the rest.  HBM-bound at few rows, by
 // the matrix and softmax units at many: 24 sequences of 1000 to 12000 tokens, 40 to
-// 64 nodes, 64 / 8 heads of 128, bf16: 257 us with the merge's 20, 690 TFLOP/s (a large
+// 64 nodes, 64 / 8 heads of 128, bf16: 255 to 265 us with the merge's 20, 670 to 695 TFLOP/s (a large
 // library product reaches 1200), matrix units 36 % busy.
 template <int D, int NQT, int WAVES, bool FINE>
 __global__ __launch_bounds__(64 * WAVES, (D > 128 && WAVES == 4 ? 1 : 2)) void tree_wide_kernel(PlanArg plan, TreeArgs a) {
