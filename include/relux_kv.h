@@ -408,7 +408,8 @@ int32_t rlx_rope(void *cache, int64_t rows, int32_t heads, int32_t head_dim, int
  * q, out and the rest as for rlx_gqa_attend, but out must not overlap q.  f32
  * queries, or f32 outputs, are computed as exactly as f32; bf16 both ways rounds
  * the softmax weights to bf16.  A call whose keys are cut takes workspace for its
- * partial sums (see rlx_cache_reserve). */
+ * partial sums (see rlx_cache_reserve).  A captured call has at most 64 sequences
+ * and comes after the append that follows a rollback (RLX_ERR_STATE otherwise). */
 int32_t rlx_gqa_attend_tree(void *cache, int32_t layer, int32_t n_seqs, const int32_t *seq_ids,
                             const int32_t *n_nodes, const int32_t *n_q, int32_t num_heads,
                             const void *q, int32_t q_dtype, int32_t qo_layout, float scale,
@@ -418,7 +419,8 @@ int32_t rlx_gqa_attend_tree(void *cache, int32_t layer, int32_t n_seqs, const in
  * one sequence after the other) stay, moved together behind the tokens before
  * the tree, and the rest is rolled back (layer -1: every layer).  Cache bytes,
  * tables, free lists and append history are then those of an append of the kept
- * tokens alone.  GQA caches.  Validated in full before any change. */
+ * tokens alone.  GQA caches.  Validated in full before any change; not to be
+ * captured (the path is the host's). */
 int32_t rlx_keep_path(void *cache, int32_t layer, int32_t n_seqs, const int32_t *seq_ids,
                       const int32_t *n_nodes, const int32_t *n_keep, const int32_t *path);
 
@@ -589,7 +591,8 @@ int32_t rlx_spec_accept_async(void *cache, const float *draft_logits, const floa
  * the accepted nodes from the root on, then -1; n_accepted and next_token device
  * int32 [n_seqs].  Rows without probability mass (NaN) give some token of the
  * vocabulary.  Sampler fields besides the temperature must be off
- * (RLX_ERR_UNSUPPORTED).  Enqueued on the cache's stream without waiting. */
+ * (RLX_ERR_UNSUPPORTED).  Enqueued on the cache's stream without waiting; a
+ * captured call has at most 256 sequences. */
 int32_t rlx_tree_accept_async(void *cache, const float *target_logits, int64_t target_stride,
                               const float *draft_logits, int64_t draft_stride, const int32_t *tokens,
                               const int32_t *parents, int32_t n_seqs, const int32_t *n_nodes,

@@ -3229,6 +3229,12 @@ int32_t rlx_spec_accept(void *h, const float *draft_logits, const float *target_
 
 // ---- trees of drafts ---------------------------------------------------------
 
+// A graph would copy a staging buffer, whose contents change, at every replay.
+static int32_t eager_only(Cache *c, const char *entry, const char *what) {
+    if (!capturing(c)) return RLX_OK;
+    return fail(RLX_ERR_STATE, "%s: %s cannot be captured", entry, what);
+}
+
 static bool is_dtype(int32_t t) { return t == RLX_F32 || t == RLX_BF16; }
 
 int32_t rlx_rope(void *h, int64_t rows, int32_t heads, int32_t head_dim, int32_t rotary_dim, const void *x,
@@ -3338,12 +3344,16 @@ static int32_t attend_tree_impl(Cache *c, int32_t layer, int32_t n_seqs, const i
     rows.swap(by_cut);
     if (wgs > 0x7FFFFFFF) return fail(RLX_ERR_UNSUPPORTED, "rlx_gqa_attend_tree: %lld work-groups", (long long)wgs);
     int32_t rc;
+    const bool args = rows.size() * sizeof(TreeRow) <= sizeof(PlanArg);
+    if (!c->pending.empty() && (rc = eager_only(c, "rlx_gqa_attend_tree", "table writes not yet on the device")))
+        return rc;
+    if (!args && (rc = eager_only(c, "rlx_gqa_attend_tree", "a call of more than 64 sequences"))) return rc;
     if ((rc = flush_patches(c))) return rc;
     const size_t po = (size_t)parts * qt * c->hd * sizeof(float), pm = (size_t)parts * qt * 2 * sizeof(float);
     if ((rc = ensure_ws(c, po + pm))) return rc;
     PlanArg plan;
     TreeArgs a{};
-    if (rows.size() * sizeof(TreeRow) <= sizeof plan) {
+    if (args) {
         memcpy(plan.b, rows.data(), rows.size() * sizeof(TreeRow));
     } else {
         std::vector<int32_t> work;
@@ -3456,6 +3466,7 @@ int32_t rlx_keep_path(void *h, int32_t layer, int32_t n_seqs, const int32_t *seq
             for (int j = p0; j < m; j++) moves.push_back(path[at + j] - p0);
         }
         if (!rows.empty()) {
+            if ((rc = eager_only(c, "rlx_keep_path", "moving nodes"))) return rc;
             if ((rc = flush_patches(c))) return rc;
             Blob b;
             const size_t o_r = b.add(rows), o_p = b.add(moves);
@@ -3520,7 +3531,9 @@ int32_t rlx_tree_accept_async(void *h, const float *target_logits, int64_t targe
             memcpy(plan.b, trees.data(), trees.size() * sizeof(int2));
         } else {
             void *dev;
-            const int32_t rc = stage(c, trees.data(), trees.size() * sizeof(int2), &dev);
+            int32_t rc = eager_only(c, "rlx_tree_accept_async", "a call of more than 256 sequences");
+            if (rc) return rc;
+            rc = stage(c, trees.data(), trees.size() * sizeof(int2), &dev);
             if (rc) return rc;
             a.trees = (const int2 *)dev;
         }

@@ -418,7 +418,6 @@ class KVCache(_PagedCache):
                                                _dtype_code(out)))
         return out
 
-
     def AttendTree(self, layer_idx, q, num_heads, parents, seq_ids=(0,), n_nodes=None, n_q=None, layout="SHD",
                    scale=None, out=None, out_dtype=torch.float32):
         """Attention of trees of drafted tokens (rlx_gqa_attend_tree).  The last

@@ -565,7 +565,7 @@ def test_refusals(gpu):
     with pytest.raises(ValueError):
         c.Rotate(x, pos, torch.ones(5, device=gpu))
     with pytest.raises(ValueError):
-        c.Rotate(x, pos, inv, layout="neox")
+        c.Rotate(x, pos, inv, layout="both")
     with pytest.raises(ValueError):
         c.Rotate(x.transpose(1, 2), pos, inv)
     with pytest.raises(TypeError):

@@ -219,3 +219,64 @@ def test_two_streams(gpu):
     for k, w in enumerate(work):
         for o in outs[k]:
             assert torch.equal(o, w[3])
+
+
+def test_what_a_graph_cannot_hold_is_refused(gpu):
+    """Staged plans, table writes under way and kept paths do not go into a graph; nothing changes."""
+    from relux_amd import KVCache, ReluxError, Sampler, tree_accept_async
+    B, H, KVH, D = 70, 2, 1, 16
+    c = KVCache(num_layers=1, max_len=64, num_kv_heads=KVH, head_dim=D, max_seqs=B, device=gpu.index)
+    k = torch.randn(B * 20, KVH, D, device=gpu)
+    c.Append(0, k, k, seq_ids=list(range(B)), n_tok=[20] * B, layout="SHD")
+    q, par = torch.randn(B * 4, H, D, device=gpu), torch.full((B * 4,), -1, dtype=torch.int32, device=gpu)
+    want = c.AttendTree(0, q, H, par, seq_ids=list(range(B)), n_nodes=[4] * B)
+    few = c.AttendTree(0, q[:4], H, par[:4])
+    t, u = torch.randn(300, 10, device=gpu), torch.rand(300, device=gpu)
+    out, stream = torch.empty_like(want), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    c.use_stream(stream)
+
+    def refused(call, match):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+            with pytest.raises(ReluxError, match=match):
+                call()
+
+    refused(lambda: c.AttendTree(0, q, H, par, seq_ids=list(range(B)), n_nodes=[4] * B, out=out), "64 sequences")
+    refused(lambda: c.KeepPath(0, 4, [0, 2]), "captured")
+    refused(lambda: tree_accept_async(c, t, torch.zeros(300, dtype=torch.int32, device=gpu), par[:300].new_zeros(300),
+                                      [1] * 300, u, Sampler()), "256 sequences")
+    c.Rollback(seq=1, n_tokens=8)  # its second page goes back: a table write under way
+    refused(lambda: c.AttendTree(0, q[:4], H, par[:4], out=out[:4]), "table writes")
+    with torch.cuda.stream(stream):
+        assert torch.equal(c.AttendTree(0, q[:4], H, par[:4]), few)
+        assert c.TotalLen(0, 0) == 20 and c.TotalLen(0, 1) == 12
+    torch.cuda.synchronize()
+    c.close()
+
+
+def test_pages_past_32_bit_offsets(gpu):
+    """A tree on pages whose byte offsets in the pools pass 2^32: attention, kept path, gather."""
+    from relux_amd import KVCache
+    g = torch.Generator(device=gpu).manual_seed(31)
+    H, KVH, D, T, n, far = 16, 8, 128, 333, 40, 9 * 2 ** 18  # 9 * 2^18 tokens of 2 KB: 4.5 GiB a pool
+    c = KVCache(num_layers=1, max_len=far, num_kv_heads=KVH, head_dim=D, max_seqs=2, pool_pages=far // 16 + 32,
+                device=gpu.index)
+    fill = torch.zeros(2 ** 18, KVH, D, device=gpu, dtype=torch.bfloat16)
+    for _ in range(9):
+        c.Append(0, fill, fill, n_tok=[2 ** 18], layout="SHD")
+    K, V = (torch.randn(T + n, KVH, D, device=gpu, generator=g).bfloat16() for _ in range(2))
+    c.Append(0, K, V, seq_ids=[1], n_tok=[T + n], layout="SHD")
+    assert min(p for p in c.PageTable(0, 1) if p >= 0) * 16 * KVH * D * 2 > 2 ** 32
+    rng = random.Random(4)
+    tree = [-1] + [rng.randint(max(0, j - 5), j - 1) for j in range(1, n)]
+    q = torch.randn(n, H, D, device=gpu, generator=g)
+    got = c.AttendTree(0, q, H, torch.tensor(tree, dtype=torch.int32, device=gpu), seq_ids=[1], n_nodes=[n])
+    want, size = ref.attend(q, K, V, tree)
+    # weights and scores in parts of bf16 as exact as f32: 2^-16 covers both
+    assert ((got.double() - want).abs() <= 4 * 2.0 ** -16 * size + 1e-7).all()
+    path = ref.ancestors(tree, n - 1)[::-1]
+    c.KeepPath(1, n, path)
+    k, v = c.View(0, 1)
+    keep = list(range(T)) + [T + j for j in path]
+    assert torch.equal(k[0].transpose(0, 1), K[keep]) and torch.equal(v[0].transpose(0, 1), V[keep])
+    c.close()
