@@ -350,9 +350,8 @@ class TreeSpeculativeDecoder:
         rows = [self.draft.forward_tree(ids, parents, depths, 1)]
         score, level = {0: 0.0}, [0]
         for width in levels:
-            order = sorted(level, key=lambda j: -score[j])
             fresh = []
-            for rank, j in enumerate(order):
+            for j in sorted(level, key=lambda j: -score[j]):
                 take = min(self.branch, width - len(fresh), rows[0].shape[1])
                 if take <= 0:
                     break
