@@ -44,7 +44,7 @@ def _fill(c, K, V, P):
 
 def _bound(want, size, dtype):
     # bf16: each weight is off by half a step, 2^-8, in the sum and in its norm, and the output by half a
-    # step.  f32: weights in two bf16 parts, 2^-16 at the worst in both, scores within 2^-16 (128 products
+    # step.  f32: weights in bf16 parts, at least two, 2^-16 at the worst in both, scores within 2^-16 (128 products
     # summed in f32) in both.
     if dtype == torch.bfloat16:
         return 2.0 ** -8 * want.abs() + 2 * 2.0 ** -8 * size + 1e-6
@@ -200,6 +200,44 @@ def test_attend_tree_in_a_graph(gpu):
         graph.replay()
         torch.cuda.synchronize()
         _check(out, [ref.attend(q, K, V, tree)], torch.bfloat16)
+    c.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [6, 70])
+def test_queries_and_outputs_off_alignment(gpu, dtype, n):
+    g = torch.Generator(device=gpu).manual_seed(n)
+    H, KVH, D, T = 8, 2, 64, 500
+    K, V = (torch.randn(T + n, KVH, D, device=gpu, generator=g).bfloat16() for _ in range(2))
+    c = _cache(gpu, KVH, D, 16, [T + n])
+    c.Append(0, K, V, n_tok=[T + n], layout="SHD")
+    par = torch.arange(-1, n - 1, dtype=torch.int32, device=gpu)
+    buf = torch.randn(n * H * D + 1, device=gpu, generator=g).to(dtype)
+    out = torch.full((n * H * D + 3,), 5.0, device=gpu, dtype=dtype)
+    c.AttendTree(0, buf[1:], H, par, out=out[1:-2])
+    assert torch.equal(out[1:-2], c.AttendTree(0, buf[1:].clone(), H, par, out_dtype=dtype))
+    assert out[0] == 5.0 and (out[-2:] == 5.0).all()
+    c.close()
+
+
+def test_tree_after_evicted_pages(gpu):
+    """A sequence whose first pages are gone: the tree attends what is left, the kept path stands behind it."""
+    g, rng = torch.Generator(device=gpu).manual_seed(6), random.Random(6)
+    H, KVH, D, T, n = 8, 4, 64, 200, 30
+    K, V = (torch.randn(T + n, KVH, D, device=gpu, generator=g).bfloat16() for _ in range(2))
+    c = _cache(gpu, KVH, D, 16, [T + n])
+    c.Append(0, K[:T], V[:T], n_tok=[T], layout="SHD")
+    c.Evict(0, 3)
+    c.Append(0, K[T:], V[T:], n_tok=[n], layout="SHD")
+    tree = _tree("random", n, rng)
+    q = torch.randn(n, H, D, device=gpu, generator=g)
+    got = c.AttendTree(0, q, H, torch.tensor(tree, dtype=torch.int32, device=gpu))
+    _check(got, [ref.attend(q, K[48:], V[48:], tree)], torch.float32)
+    path = ref.ancestors(tree, n - 1)[::-1]
+    c.KeepPath(0, n, path)
+    k, v = c.View(0)
+    keep = list(range(48, T)) + [T + j for j in path]
+    assert torch.equal(k[0].transpose(0, 1), K[keep]) and torch.equal(v[0].transpose(0, 1), V[keep])
     c.close()
 
 
