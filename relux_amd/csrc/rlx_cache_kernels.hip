@@ -250,26 +250,23 @@ hipError_t launch_mla_append(hipStream_t s, const PlanArg *plan, int tok_off, ui
 }
 
 // Paged gather of GQA K and V into dense [kvh][T][hd] per sequence.
-// grid.y = sequence of the call; x covers the sequence's work, the first v_blocks V
-// and the others K.  K: thread = (token, head, 8-dim chunk), 16-byte read and write.
-// V: 8 dims x 8 tokens a thread, turned in registers, neighbouring threads on
-// neighbouring dims of the output rows.
-// HBM-bound: 16 sequences of 105 to 305 tokens, 8 kv heads of 128: 8.3 to 10.6 us (V after
-// K in the same blocks 9.1 to 10.8, V by 2-byte stores 18.9); one of 205: 3.9 (4.5).
+// grid.y = sequence of the call; x covers the sequence's work.  K: thread =
+// (token, head, 8-dim chunk), 16-byte read and write.  V: thread = (head, dim,
+// 8-token chunk), 16-byte read of a dim-major page row, 8 strided writes.
 template <bool ARG>
 __global__ void kv_gather_kernel(typename PlanSel<ARG>::T plan, const uint16_t *__restrict__ kpool,
                                  const uint16_t *__restrict__ vpool,
                                  const int32_t *__restrict__ table, const AttRow *__restrict__ rows,
                                  uint16_t *__restrict__ k_out, uint16_t *__restrict__ v_out,
-                                 int kvh, int hd, int hdi, int P, int v_blocks) {
+                                 int kvh, int hd, int hdi, int P) {
     // Stored pages hold hd dims per head; the dense output holds the
     // caller's hdi (<= hd, a multiple of 8) and drops the zero padding.
     const AttRow R = plan_row<ARG>(rows, blockIdx.y);
     const int chunks = hdi >> 3;
     const int64_t nk = (int64_t)R.len * kvh * chunks;
     const int64_t base = (int64_t)R.qrow * kvh * hdi;  // qrow holds the output token offset
-    for (int64_t gid = (int64_t)((int)blockIdx.x - v_blocks) * blockDim.x + threadIdx.x; gid >= 0 && gid < nk;
-         gid += (int64_t)(gridDim.x - v_blocks) * blockDim.x) {
+    for (int64_t gid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; gid < nk;
+         gid += (int64_t)gridDim.x * blockDim.x) {
         const int t = (int)(gid / ((int64_t)kvh * chunks));
         const int rem = (int)(gid - (int64_t)t * kvh * chunks);
         const int h = rem / chunks;
@@ -279,11 +276,13 @@ __global__ void kv_gather_kernel(typename PlanSel<ARG>::T plan, const uint16_t *
         u32x4 v = *(const u32x4 *)(kpool + ((int64_t)page * kvh + h) * P * hd + k_page_off(slot, d0, hd));
         *(u32x4 *)(k_out + base + ((int64_t)h * R.len + t) * hdi + d0) = v;
     }
-    if ((int)blockIdx.x >= v_blocks) return;
+    // V: 8 dims x 8 tokens a thread, turned in registers, neighbouring threads on
+    // neighbouring dims of the output rows.  16 sequences of 105 to 305 tokens, 8 kv
+    // heads of 128: 18.9 us by 2-byte stores.
     const int tchunks = (R.len + 7) >> 3;
     const int64_t nv = (int64_t)kvh * tchunks * chunks;
     for (int64_t gid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; gid < nv;
-         gid += (int64_t)v_blocks * blockDim.x) {
+         gid += (int64_t)gridDim.x * blockDim.x) {
         const int64_t ht = gid / chunks;
         const int d0 = (int)(gid - ht * chunks) * 8, h = (int)(ht / tchunks), t0 = (int)(ht - (int64_t)h * tchunks) * 8;
         const int page = table[R.tab + t0 / P];
@@ -310,15 +309,15 @@ hipError_t launch_kv_gather(hipStream_t s, const PlanArg *plan, const uint16_t *
                             const int32_t *table, const AttRow *rows, int n_rows, int max_len,
                             uint16_t *k_out, uint16_t *v_out, int kvh, int hd, int hdi, int P) {
     if (n_rows <= 0 || max_len <= 0) return hipSuccess;
-    const int64_t work = (int64_t)max_len * kvh * (hd / 8);
-    const int k_blocks = (int)std::min<int64_t>((work + 255) / 256, 4096);
-    const int v_blocks = (int)std::min<int64_t>((work / 8 + 255) / 256, 4096), blocks = v_blocks + k_blocks;
+    int64_t work = (int64_t)max_len * kvh * (hd / 8);
+    int blocks = (int)((work + 255) / 256);
+    if (blocks > 4096) blocks = 4096;
     if (plan)
         kv_gather_kernel<true><<<dim3(blocks, n_rows), 256, 0, s>>>(*plan, kpool, vpool, table, rows, k_out, v_out, kvh,
-                                                                   hd, hdi, P, v_blocks);
+                                                                   hd, hdi, P);
     else
         kv_gather_kernel<false><<<dim3(blocks, n_rows), 256, 0, s>>>(NoPlan{0}, kpool, vpool, table, rows, k_out, v_out,
-                                                                    kvh, hd, hdi, P, v_blocks);
+                                                                    kvh, hd, hdi, P);
     return hipGetLastError();
 }
 
