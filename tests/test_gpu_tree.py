@@ -554,6 +554,18 @@ def test_keep_path_one_layer_and_the_step_after(gpu):
     c.close()
 
 
+@pytest.mark.parametrize("T", [1, 3, 8, 9])
+def test_gather_of_a_few_tokens(gpu, T):
+    g = torch.Generator(device=gpu).manual_seed(T)
+    for KVH, D in ((1, 16), (1, 8), (3, 64)):
+        K, V = (torch.randn(T, KVH, D, device=gpu, generator=g).bfloat16() for _ in range(2))
+        c = _cache(gpu, KVH, D, 16, [T])
+        c.Append(0, K, V, n_tok=[T], layout="SHD")
+        k, v = c.View(0)
+        assert torch.equal(k[0].transpose(0, 1), K) and torch.equal(v[0].transpose(0, 1), V)
+        c.close()
+
+
 # ---- refusals ----------------------------------------------------------------------------------
 
 def test_refusals(gpu):
