@@ -139,7 +139,7 @@ struct RowStat {
 // once the node before it is decided.  Bound by that chain of passes, at most one a
 // node of the path and one a rejection: V / 4 entries a SIMD, half of the time their
 // exponentials and sums, half a row's latency and the joins.  64 trees of 32 nodes, 32000
-// tokens: 45 to 50 us, up to 7 passes; 12 of 9 to 61, 50257 tokens: 63 to 70 us; one of 8
+// tokens: 45 to 52 us, up to 7 passes; 12 of 9 to 61, 50257 tokens: 63 to 70 us; one of 8
 // without draft logits, 32000 tokens: 13 us.  16 waves: 8 take 46 and 64 us, 4 take 69 and 91;
 // batches of 8 loads instead of 4, 62 and 76.  Weights of 16 float4 a lane kept in
 // registers between passes: 43 and 67, for a second form of every pass.
